@@ -210,6 +210,67 @@ int qtts_paged_attention_noalloc(const void* q, int R, int num_heads, int kv_hea
                                  const int32_t* row_slot, const int32_t* row_ctx, int max_ctx,
                                  void* out, void* out_lo, qtts_stream_t stream);
 
+/* ---- 4-bit KV cache ------------------------------------------------------------
+ * A pool in 4.5 bits an element beside the fp16 one (which holds 16).  Groups of 64 channels of
+ * one token, head and k|v share an fp16 scale and zero:
+ *   zero = fp16(min), scale = fp16((max - min) * fp32(1/15)) (fp32 steps), values saturated to
+ *   +-65504 first; code = nearest integer to fp32(x - zero) / scale (exact quotient, ties to
+ *   even), clamped to [0, 15], 0 where scale = 0;  value = code * scale + zero.
+ * A NaN makes its group read back as NaN.
+ * Layout: [num_blocks][num_layers][2][kv_heads] chunks of QTTS_Q4_CHUNK_BYTES(head_dim) bytes, a
+ * chunk = 16 tokens: 16 rows of head_dim / 2 bytes of codes, whose 32-bit words alternate between
+ * the row's NG = head_dim / 64 groups (word NG * i + w = channels 64 w + 8 i .. + 7, the first in the
+ * low nibble), then [NG][16 tokens] (scale, zero) fp16 pairs.  A block is contiguous, so
+ * qtts_kv_copy_blocks copies it (block_elems = bytes / 2).  head_dim 64 or 128, block_size 16;
+ * the pool must be 16-byte aligned.  Keys of a pool that was zero-filled read as zeros. */
+#define QTTS_Q4_CHUNK_BYTES(head_dim) ((head_dim) * 8 + (head_dim))
+#define QTTS_F16  0
+#define QTTS_BF16 1
+#define QTTS_F32  2
+
+/* Quantise the K and V rows of n tokens and n_layers layers (from first_layer) into the pool
+ * positions slot_mapping[n] (block * 16 + offset; negative or past the pool: skipped), as the
+ * tokens of a step are written.  k, v: elements of `dtype` (QTTS_F16 / BF16 / F32), channels
+ * contiguous; k_strides, v_strides: element strides of (token, layer, head), host arrays of 3.
+ * The positions of one call must differ: of two tokens written to one position, the cache keeps a
+ * mixture. */
+int qtts_kv_write_q4(void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim, const void* k,
+                     const void* v, int dtype, const int64_t* k_strides, const int64_t* v_strides, int first_layer,
+                     int n_layers, const int32_t* slot_mapping, int n, qtts_stream_t stream);
+/* The inverse: what the positions hold, written to k and v (same arguments; a position outside the
+ * pool reads as zeros). */
+int qtts_kv_read_q4(const void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim, void* k, void* v,
+                    int dtype, const int64_t* k_strides, const int64_t* v_strides, int first_layer, int n_layers,
+                    const int32_t* slot_mapping, int n, qtts_stream_t stream);
+/* qtts_kv_gather for a 4-bit pool: the first n_tokens tokens of a block list (a block-table row or a
+ * prefix entry, device int32), out [layers*2][kv_heads][n_tokens][head_dim] fp16; ids outside the
+ * pool read as zeros. */
+int qtts_kv_gather_q4(const void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim,
+                      const int32_t* blocks, int n_tokens, void* out, qtts_stream_t stream);
+
+/* Paged attention under a sliding window with sinks: a row of row_ctx = c keys sees key j when
+ *   j < c and (j >= c - window or j < sinks or window == 0)
+ * and gets softmax(q k^T / sqrt(head_dim)) v over those; a row that sees none (c <= 0) gets zeros.
+ * Only blocks that hold a visible key are read, and what a row does not see (stale entries,
+ * NaN, infinity) does not reach it.  fp16 pool as qtts_paged_attention; head_dim 64 or 128, any
+ * whole number of query heads per KV head; row_ctx is capped at max_ctx.  rows_per_stream: as
+ * qtts_paged_attention_prefill (R / rows_per_stream streams of consecutive query rows that share
+ * row_slot; 1 = decode rows).  block_table [num_slots][max_blocks_per_seq]; a row_slot outside
+ * [0, num_slots) gives zeros, a block id outside the pool hides its keys; both are reported by
+ * qtts_device_error.  q and kv_pool must be 16-byte aligned.  No scratch: keys of few rows are split
+ * over the CTAs of a cluster and folded through distributed shared memory, in a fixed order. */
+int qtts_paged_attention_window(const void* q, int R, int rows_per_stream, int num_heads, int kv_heads, int head_dim,
+                                const void* kv_pool, int layer, int num_layers, int block_size, int num_blocks,
+                                const int32_t* block_table, int num_slots, int max_blocks_per_seq,
+                                const int32_t* row_slot, const int32_t* row_ctx, int max_ctx, int window, int sinks,
+                                void* out, void* out_lo, qtts_stream_t stream);
+/* The same attention over a 4-bit pool. */
+int qtts_paged_attention_q4(const void* q, int R, int rows_per_stream, int num_heads, int kv_heads, int head_dim,
+                            const void* cache, int layer, int num_layers, int block_size, int num_blocks,
+                            const int32_t* block_table, int num_slots, int max_blocks_per_seq,
+                            const int32_t* row_slot, const int32_t* row_ctx, int max_ctx, int window, int sinks,
+                            void* out, void* out_lo, qtts_stream_t stream);
+
 /* Top-k / temperature / Gumbel-max sampling of fp32 logits [R][V] (row stride ld).
  * Talker head (talker_unified_modules.py:373-388) when counts != NULL: suppress
  * [V-1024,V) except eos_id, repetition penalty on counts>0, counts[tok] += 1.

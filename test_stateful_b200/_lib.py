@@ -27,6 +27,7 @@ ERR_UNSUPPORTED = -6
 
 EPI_BF16, EPI_F32, EPI_RESIDUAL, EPI_SWIGLU, EPI_QKV_ROPE = range(5)
 ATTN_SPLIT_BLOCKS = 16
+DT_F16, DT_BF16, DT_F32 = range(3)
 
 _STATUS_NAMES = {ERR_INVALID: "invalid argument", ERR_CUDA: "CUDA error", ERR_CAPACITY: "sequence capacity",
                  ERR_POOL_EXHAUSTED: "KV pool exhausted", ERR_TIMEOUT: "device wait timed out",
@@ -100,7 +101,8 @@ EXPORTS = [
     "qtts_sched_init", "qtts_sched_append", "qtts_kv_copy_blocks", "qtts_sched_share_prefix",
     "qtts_sched_make_entry", "qtts_sched_drop_blocks", "qtts_sched_release", "qtts_kv_scatter", "qtts_kv_gather",
     "qtts_gemm", "qtts_rmsnorm", "qtts_paged_attention", "qtts_paged_attention_prefill",
-    "qtts_paged_attention_noalloc", "qtts_sample",
+    "qtts_paged_attention_noalloc", "qtts_kv_write_q4", "qtts_kv_read_q4", "qtts_kv_gather_q4",
+    "qtts_paged_attention_window", "qtts_paged_attention_q4", "qtts_sample",
     "qtts_philox_gumbel", "qtts_codec_sum",
     "qtts_engine_create", "qtts_engine_destroy", "qtts_engine_step",
     "qtts_c2w_create", "qtts_c2w_destroy", "qtts_c2w_reset", "qtts_c2w_step", "qtts_c2w_launches",
@@ -151,6 +153,17 @@ def load() -> C.CDLL:
                                          C.c_int),
         "qtts_paged_attention_noalloc": ([P, C.c_int, C.c_int, C.c_int, C.c_int, P, C.c_int, C.c_int, C.c_int,
                                           C.c_int, P, C.c_int, P, P, C.c_int, P, P, P], C.c_int),
+        "qtts_kv_write_q4": ([P, C.c_int, C.c_int, C.c_int, C.c_int, P, P, C.c_int, C.POINTER(C.c_int64),
+                              C.POINTER(C.c_int64), C.c_int, C.c_int, P, C.c_int, P], C.c_int),
+        "qtts_kv_read_q4": ([P, C.c_int, C.c_int, C.c_int, C.c_int, P, P, C.c_int, C.POINTER(C.c_int64),
+                             C.POINTER(C.c_int64), C.c_int, C.c_int, P, C.c_int, P], C.c_int),
+        "qtts_kv_gather_q4": ([P, C.c_int, C.c_int, C.c_int, C.c_int, P, C.c_int, P, P], C.c_int),
+        "qtts_paged_attention_window": ([P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P, C.c_int, C.c_int,
+                                         C.c_int, C.c_int, P, C.c_int, C.c_int, P, P, C.c_int, C.c_int, C.c_int,
+                                         P, P, P], C.c_int),
+        "qtts_paged_attention_q4": ([P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P, C.c_int, C.c_int,
+                                     C.c_int, C.c_int, P, C.c_int, C.c_int, P, P, C.c_int, C.c_int, C.c_int,
+                                     P, P, P], C.c_int),
         "qtts_sample": ([P, C.c_int, C.c_int, C.c_int, C.c_int, P, C.c_int, C.c_uint64, P, C.c_int, P, P, P,
                          C.c_int, P, C.c_int, P], C.c_int),
         "qtts_philox_gumbel": ([C.c_uint64, P, P, C.c_int, C.c_int, C.c_int, P, P], C.c_int),

@@ -1,0 +1,318 @@
+// 4-bit paged KV cache: quantising K/V rows as they are written, and reading them back.
+//
+// A group is 64 channels of one token and head.  With lo, hi its smallest and largest value
+// (saturated to fp16's range, +-65504):
+//   zero  = fp16(lo)
+//   scale = fp16(fl(fl(hi - lo) * fl(1/15)))
+//   code  = the integer in [0, 15] nearest to fl(x - zero) / scale, ties to even (0 when scale = 0)
+//   value = code * scale + zero
+// fl() is fp32 rounding; the quotient is taken exactly, so that the codes do not depend on how a
+// division rounds.  A NaN makes its group read back as NaN (zero = NaN, scale = 0, codes 0).
+//
+// Pool: [num_blocks][layers][2][kv_heads] chunks of 16 tokens.  A chunk is 16 rows of
+// head_dim / 2 bytes of codes, then head_dim / 64 arrays of 16 (scale, zero) fp16 pairs.  A row's
+// 32-bit words alternate between its groups (word NG * i + w holds channels 64 w + 8 i .. + 7,
+// channel 0 in the low nibble), so that one 16- or 8-byte load of the attention kernel brings a
+// lane channels of every group.
+#pragma once
+
+#include "common.cuh"
+
+namespace qtts {
+
+template <int D>
+struct Q4Layout {
+    static constexpr int NG = D / 64;                // groups per row
+    static constexpr int ROW = D / 2;                // bytes of codes per token
+    static constexpr int PARAMS = 16 * ROW;          // offset of the (scale, zero) pairs
+    static constexpr int CHUNK = PARAMS + NG * 64;   // bytes per (block, layer, k|v, head)
+};
+
+// n / d for n < 2^31 as a multiply-high and a shift (one per row instead of a hardware division)
+struct FastDiv {
+    uint32_t mul, shift, d;
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+inline FastDiv make_fastdiv(uint32_t d) {
+    FastDiv f = {0, 0, d};
+    if (d > 1) {
+        uint32_t l = 0;
+        while ((1u << l) < d) ++l;  // 2^(l-1) < d <= 2^l
+        // m = ceil(2^(31+l) / d) < 2^32 is exact for n < 2^31 (the excess e = m d - 2^(31+l) is below
+        // d <= 2^l, so n e < 2^(31+l) and the quotient is never one too high)
+        f.mul = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
+        f.shift = l - 1;
+    }
+    return f;
+}
+
+struct Q4IoParams {
+    uint8_t* cache;
+    const void *k_in, *v_in;            // write: rows in
+    void *k_out, *v_out;                // read: rows out
+    long long ks[3], vs[3];             // element strides of (token, layer, head)
+    int num_blocks, num_layers, kv_heads, first_layer;
+    int n;                              // tokens
+    const int32_t* mapping;             // position of each token (block * 16 + offset) ...
+    const int32_t* blocks;              // ... or the block id of each 16 tokens
+    FastDiv rows, heads;                // rows of one token (layers * 2 * heads), heads
+    uint32_t total;                     // ceil(n / 16) * 16 * rows
+};
+
+template <typename T>
+__device__ __forceinline__ float q4_to_float(T x);
+template <>
+__device__ __forceinline__ float q4_to_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float q4_to_float<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float q4_to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T q4_from_float(float x);
+template <>
+__device__ __forceinline__ float q4_from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half q4_from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 q4_from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// min / max that return NaN when either argument is NaN
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Where thread group `flat` works: rows are ordered 16 tokens innermost, then head, k|v, layer, then
+// the next 16 tokens, so that consecutive rows of a whole block fill a chunk.
+struct Q4Row {
+    int token, layer, kv, head;
+};
+__device__ __forceinline__ Q4Row q4_row(const Q4IoParams& p, uint32_t flat) {
+    const uint32_t t16 = flat & 15, rest = flat >> 4;
+    const uint32_t tg = p.rows.div(rest);
+    const uint32_t row = rest - tg * p.rows.d;
+    const uint32_t lk = p.heads.div(row);
+    return {(int)(tg * 16 + t16), (int)(lk >> 1), (int)(lk & 1), (int)(row - lk * p.heads.d)};
+}
+
+// Chunk address of a row's token, or NULL for a position outside the pool.
+template <int D>
+__device__ __forceinline__ uint8_t* q4_chunk(const Q4IoParams& p, const Q4Row& r, int* off) {
+    int blk;
+    if (p.mapping) {
+        const int m = __ldg(p.mapping + r.token);
+        if (m < 0) return nullptr;
+        blk = m >> 4;
+        *off = m & 15;
+    } else {
+        blk = __ldg(p.blocks + (r.token >> 4));
+        *off = r.token & 15;
+    }
+    if (blk < 0 || blk >= p.num_blocks) return nullptr;
+    const size_t c = (((size_t)blk * p.num_layers + p.first_layer + r.layer) * 2 + r.kv) * p.kv_heads + r.head;
+    return p.cache + c * Q4Layout<D>::CHUNK;
+}
+
+// Eight threads a row, thread i taking the channels 64 w + 8 i .. + 7 of every group w.
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(256) kv_write_q4_kernel(const Q4IoParams p) {
+    using L = Q4Layout<D>;
+    griddep_wait();
+    griddep_launch();
+    const uint32_t flat = blockIdx.x * 32u + (threadIdx.x >> 3);
+    const int i = threadIdx.x & 7;
+    const bool in_range = flat < p.total;
+    const Q4Row r = q4_row(p, in_range ? flat : 0);
+    int off = 0;
+    uint8_t* chunk = in_range && r.token < p.n ? q4_chunk<D>(p, r, &off) : nullptr;
+    const unsigned peers = 0xffu << (threadIdx.x & 24);  // the row's eight threads go together
+    if (!chunk) return;
+    const long long* st = r.kv ? p.vs : p.ks;
+    const T* src = reinterpret_cast<const T*>(r.kv ? p.v_in : p.k_in) + r.token * st[0] + r.layer * st[1] +
+                   r.head * st[2] + 8 * i;
+    T x[L::NG][8];
+#pragma unroll
+    for (int w = 0; w < L::NG; ++w) {
+        if constexpr (VEC) {
+            const uint4* s4 = reinterpret_cast<const uint4*>(src + 64 * w);
+#pragma unroll
+            for (int c = 0; c < (int)sizeof(T) / 2; ++c) reinterpret_cast<uint4*>(x[w])[c] = __ldg(s4 + c);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[w][c] = src[64 * w + c];
+        }
+    }
+    uint32_t word[L::NG];
+#pragma unroll
+    for (int w = 0; w < L::NG; ++w) {
+        float f[8], lo, hi;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            f[c] = q4_to_float<T>(x[w][c]);
+            lo = c ? min_nan(lo, f[c]) : f[c];
+            hi = c ? max_nan(hi, f[c]) : f[c];
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            lo = min_nan(lo, __shfl_xor_sync(peers, lo, o));
+            hi = max_nan(hi, __shfl_xor_sync(peers, hi, o));
+        }
+        const bool nan = lo != lo;
+        lo = __fadd_rn(fminf(fmaxf(lo, -65504.f), 65504.f), 0.f);  // of zeros of both signs, +0
+        hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+        const __half zero_h = nan ? __ushort_as_half(0x7fff) : __float2half_rn(lo);
+        const __half scale_h = nan ? __float2half_rn(0.f)
+                                   : __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+        const float zero = __half2float(zero_h), scale = __half2float(scale_h);
+        // t = quotient / 15, saturated to [0, 1] (NaN -> 0), then 15 t rounded to an integer by
+        // adding 2^23 + 2^22: its bits hold the code.  The reciprocal puts 15 t off by at most
+        // 2^-19; where it lands that close to a border the code is decided by exact remainders.
+        constexpr float kMagic = 12582912.f;  // 0x4B400000
+        const float inv15 = scale > 0.f ? __frcp_rn(scale) * (1.0f / 15.0f) : 0.f;
+        uint32_t acc = 0;
+        float worst = 0.f;
+        float d[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            d[c] = __fsub_rn(f[c], zero);
+            const float t = __saturatef(d[c] * inv15);
+            const float m = __fmaf_rn(t, 15.f, kMagic);
+            worst = fmaxf(worst, fabsf(__fmaf_rn(t, 15.f, kMagic - m)));
+            acc += __float_as_uint(m) << (4 * c);
+        }
+        acc -= 0x3F400000u;  // what the constant's own bits added up to, modulo 2^32
+        if (worst > 0.499995f) {
+            acc = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float t = __saturatef(d[c] * inv15);
+                int code = (int)rintf(t * 15.f);
+                // e = d - code * scale is exact wherever it is near scale / 2
+                const float e = __fmaf_rn(-(float)code, scale, d[c]), h = 0.5f * scale;
+                const bool odd = code & 1;
+                if (e > h || (e == h && odd)) ++code;
+                else if (e < -h || (e == -h && odd)) --code;
+                acc |= (uint32_t)min(max(code, 0), 15) << (4 * c);
+            }
+        }
+        word[w] = acc;
+        if (i == w)  // one thread of the row writes each group's parameters
+            *reinterpret_cast<__half2*>(chunk + L::PARAMS + w * 64 + off * 4) = __halves2half2(scale_h, zero_h);
+    }
+    uint8_t* dst = chunk + off * L::ROW + i * 4 * L::NG;
+    if constexpr (L::NG == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = word[0];
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(256) kv_read_q4_kernel(const Q4IoParams p) {
+    using L = Q4Layout<D>;
+    griddep_wait();
+    griddep_launch();
+    const uint32_t flat = blockIdx.x * 32u + (threadIdx.x >> 3);
+    const int i = threadIdx.x & 7;
+    if (flat >= p.total) return;
+    const Q4Row r = q4_row(p, flat);
+    if (r.token >= p.n) return;
+    int off = 0;
+    const uint8_t* chunk = q4_chunk<D>(p, r, &off);
+    const long long* st = r.kv ? p.vs : p.ks;
+    T* dst = reinterpret_cast<T*>(r.kv ? p.v_out : p.k_out) + r.token * st[0] + r.layer * st[1] + r.head * st[2] +
+             8 * i;
+    uint32_t word[L::NG] = {};
+    __half2 prm[L::NG];
+#pragma unroll
+    for (int w = 0; w < L::NG; ++w) prm[w] = __halves2half2(__float2half(0.f), __float2half(0.f));
+    if (chunk) {  // a position outside the pool reads as zeros
+        const uint8_t* src = chunk + off * L::ROW + i * 4 * L::NG;
+        if constexpr (L::NG == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(src);
+            word[0] = u.x;
+            word[1] = u.y;
+        } else {
+            word[0] = *reinterpret_cast<const uint32_t*>(src);
+        }
+#pragma unroll
+        for (int w = 0; w < L::NG; ++w)
+            prm[w] = *reinterpret_cast<const __half2*>(chunk + L::PARAMS + w * 64 + off * 4);
+    }
+#pragma unroll
+    for (int w = 0; w < L::NG; ++w) {
+        const float scale = __low2float(prm[w]), zero = __high2float(prm[w]);
+        T y[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            y[c] = q4_from_float<T>(__fmaf_rn((float)((word[w] >> (4 * c)) & 15u), scale, zero));
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < (int)sizeof(T) / 2; ++c)
+                reinterpret_cast<uint4*>(dst + 64 * w)[c] = reinterpret_cast<const uint4*>(y)[c];
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) dst[64 * w + c] = y[c];
+        }
+    }
+}
+
+// 16-byte accesses: the base and every stride must keep rows 16-byte aligned
+inline bool q4_vec_ok(const void* k, const void* v, const long long* ks, const long long* vs, int elem) {
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return false;
+    for (int s = 0; s < 3; ++s)
+        if ((ks[s] * elem) & 15 || (vs[s] * elem) & 15) return false;
+    return true;
+}
+
+template <typename T, int D, bool WRITE>
+inline int launch_q4_io(const Q4IoParams& p, cudaStream_t st) {
+    const bool vec = q4_vec_ok(WRITE ? p.k_in : p.k_out, WRITE ? p.v_in : p.v_out, p.ks, p.vs, (int)sizeof(T));
+    const dim3 grid((p.total + 31) / 32), block(256);
+    if constexpr (WRITE) {
+        if (vec) QTTS_LAUNCH((kv_write_q4_kernel<T, D, true>), grid, block, 0, st, p);
+        else QTTS_LAUNCH((kv_write_q4_kernel<T, D, false>), grid, block, 0, st, p);
+    } else {
+        if (vec) QTTS_LAUNCH((kv_read_q4_kernel<T, D, true>), grid, block, 0, st, p);
+        else QTTS_LAUNCH((kv_read_q4_kernel<T, D, false>), grid, block, 0, st, p);
+    }
+    return QTTS_OK;
+}
+
+template <bool WRITE>
+inline int run_q4_io(Q4IoParams p, int layers, int head_dim, int dtype, cudaStream_t st) {
+    const long long per_token = (long long)layers * 2 * p.kv_heads;
+    QTTS_REQUIRE(per_token <= (1 << 20), "q4 cache: %lld rows per token", per_token);
+    p.rows = make_fastdiv((uint32_t)per_token);
+    p.heads = make_fastdiv((uint32_t)p.kv_heads);
+    // row numbers stay below 2^31: longer inputs go in several launches
+    const int step = (int)(((1ll << 30) / per_token) & ~15ll);
+    const int n = p.n, elem = dtype == QTTS_F32 ? 4 : 2;
+    for (int t0 = 0; t0 < n; t0 += step) {
+        Q4IoParams c = p;
+        c.n = n - t0 < step ? n - t0 : step;
+        c.total = (uint32_t)((c.n + 15) / 16 * 16 * per_token);
+        if (c.mapping) c.mapping += t0;
+        if (c.blocks) c.blocks += t0 / 16;
+        const long long ko = (long long)t0 * p.ks[0] * elem, vo = (long long)t0 * p.vs[0] * elem;
+        if (WRITE) {
+            c.k_in = (const char*)p.k_in + ko;
+            c.v_in = (const char*)p.v_in + vo;
+        } else {
+            c.k_out = (char*)p.k_out + ko;
+            c.v_out = (char*)p.v_out + vo;
+        }
+        int rc = QTTS_OK;
+        if (dtype == QTTS_F16) rc = head_dim == 128 ? launch_q4_io<__half, 128, WRITE>(c, st) : launch_q4_io<__half, 64, WRITE>(c, st);
+        else if (dtype == QTTS_BF16) rc = head_dim == 128 ? launch_q4_io<__nv_bfloat16, 128, WRITE>(c, st) : launch_q4_io<__nv_bfloat16, 64, WRITE>(c, st);
+        else rc = head_dim == 128 ? launch_q4_io<float, 128, WRITE>(c, st) : launch_q4_io<float, 64, WRITE>(c, st);
+        if (rc) return rc;
+    }
+    return QTTS_OK;
+}
+
+}  // namespace qtts

@@ -8,6 +8,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "attn_window.cuh"
 #include "code2wav.cuh"
 #include "engine.cuh"
 
@@ -25,6 +26,85 @@ void set_error(const char* fmt, ...) {
 static bool state_ok(const qtts_paged_state* s) {
     return s && s->free_stack && s->free_top && s->refcount && s->block_table && s->seq_len && s->position_offset &&
            s->num_blocks > 0 && s->block_size == 16 && s->max_slots > 0 && s->max_blocks_per_seq > 0;
+}
+
+// pool geometry and rows of the 4-bit cache entries
+static int q4_io_check(const char* what, const void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim,
+                       const void* k, const void* v, int dtype, const int64_t* ks, const int64_t* vs, int first_layer,
+                       int n_layers, const int32_t* index, int n) {
+    QTTS_REQUIRE(n >= 0, "%s: n %d", what, n);
+    QTTS_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim %d (64 or 128)", what, head_dim);
+    QTTS_REQUIRE(num_blocks > 0 && num_blocks <= (1 << 27) && num_layers > 0 && kv_heads > 0,
+                 "%s: empty or oversized pool", what);
+    QTTS_REQUIRE(first_layer >= 0 && n_layers > 0 && n_layers <= num_layers && first_layer <= num_layers - n_layers,
+                 "%s: layers [%d, +%d) of %d", what, first_layer, n_layers, num_layers);
+    QTTS_REQUIRE(dtype == QTTS_F16 || dtype == QTTS_BF16 || dtype == QTTS_F32, "%s: dtype %d", what, dtype);
+    if (n == 0) return QTTS_OK;
+    QTTS_REQUIRE(cache && k && v && ks && vs && index, "%s: null pointer", what);
+    const uintptr_t elem = dtype == QTTS_F32 ? 4 : 2;
+    QTTS_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0 && (reinterpret_cast<uintptr_t>(index) & 3) == 0 &&
+                     ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & (elem - 1)) == 0,
+                 "%s: misaligned pointer", what);
+    return QTTS_OK;
+}
+
+static Q4IoParams q4_io_params(const void* cache, int num_blocks, int num_layers, int kv_heads, const int64_t* ks,
+                               const int64_t* vs, int first_layer, int n) {
+    Q4IoParams p = {};
+    p.cache = reinterpret_cast<uint8_t*>(const_cast<void*>(cache));
+    p.num_blocks = num_blocks;
+    p.num_layers = num_layers;
+    p.kv_heads = kv_heads;
+    p.first_layer = first_layer;
+    p.n = n;
+    for (int i = 0; i < 3; ++i) p.ks[i] = ks[i], p.vs[i] = vs[i];
+    return p;
+}
+
+static int window_attention(const char* what, int fmt, const void* q, int R, int rows_per_stream, int num_heads,
+                            int kv_heads, int head_dim, const void* kv, int layer, int num_layers, int block_size,
+                            int num_blocks, const int32_t* block_table, int num_slots, int mbps,
+                            const int32_t* row_slot, const int32_t* row_ctx, int max_ctx, int window, int sinks,
+                            void* out, void* out_lo, cudaStream_t st) {
+    QTTS_REQUIRE(R >= 0 && rows_per_stream >= 1 && R % rows_per_stream == 0, "%s: %d rows are not streams of %d tokens",
+                 what, R, rows_per_stream);
+    QTTS_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim %d (64 or 128)", what, head_dim);
+    QTTS_REQUIRE(block_size == 16, "%s: block_size must be 16", what);
+    QTTS_REQUIRE(kv_heads > 0 && num_heads > 0 && num_heads % kv_heads == 0,
+                 "%s: %d query heads over %d kv heads", what, num_heads, kv_heads);
+    QTTS_REQUIRE(num_layers > 0 && layer >= 0 && layer < num_layers && num_blocks > 0 && num_slots > 0,
+                 "%s: layer or pool out of range", what);
+    QTTS_REQUIRE(mbps > 0 && mbps <= (1 << 26) && max_ctx > 0 && max_ctx <= mbps * 16, "%s: max_ctx out of range", what);
+    QTTS_REQUIRE(window >= 0 && sinks >= 0, "%s: negative window or sinks", what);
+    if (R == 0) return QTTS_OK;
+    QTTS_REQUIRE(q && kv && block_table && row_slot && row_ctx && out, "%s: null pointer", what);
+    QTTS_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv)) & 15) == 0,
+                 "%s: q and the pool must be 16-byte aligned", what);
+    WinParams p = {};
+    p.q = reinterpret_cast<const float*>(q);
+    p.kv = reinterpret_cast<const uint8_t*>(kv);
+    p.block_table = block_table;
+    p.row_slot = row_slot;
+    p.row_ctx = row_ctx;
+    p.out = reinterpret_cast<__nv_bfloat16*>(out);
+    p.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
+    p.R = R;
+    p.S = rows_per_stream;
+    p.num_heads = num_heads;
+    p.kv_heads = kv_heads;
+    p.group = num_heads / kv_heads;
+    p.layer = layer;
+    p.num_layers = num_layers;
+    p.num_blocks = num_blocks;
+    p.num_slots = num_slots;
+    p.mbps = mbps;
+    p.max_ctx = max_ctx;
+    p.window = window;
+    p.sinks = sinks;
+    p.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
+    if (fmt == kWinQ4)
+        return head_dim == 128 ? launch_window_attention<kWinQ4, 128>(p, st) : launch_window_attention<kWinQ4, 64>(p, st);
+    return head_dim == 128 ? launch_window_attention<kWinF16, 128>(p, st) : launch_window_attention<kWinF16, 64>(p, st);
 }
 
 }  // namespace qtts
@@ -236,6 +316,69 @@ int qtts_paged_attention_prefill(const void* q, int R, int rows_per_stream, int 
     p.R = R;
     p.rows_per_stream = rows_per_stream;
     return launch_prefill_attention(p, (cudaStream_t)stream);
+}
+
+int qtts_kv_write_q4(void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim, const void* k,
+                     const void* v, int dtype, const int64_t* k_strides, const int64_t* v_strides, int first_layer,
+                     int n_layers, const int32_t* slot_mapping, int n, qtts_stream_t stream) {
+    const int rc = q4_io_check("kv_write_q4", cache, num_blocks, num_layers, kv_heads, head_dim, k, v, dtype, k_strides,
+                               v_strides, first_layer, n_layers, slot_mapping, n);
+    if (rc || n == 0) return rc;
+    Q4IoParams p = q4_io_params(cache, num_blocks, num_layers, kv_heads, k_strides, v_strides, first_layer, n);
+    p.k_in = k;
+    p.v_in = v;
+    p.mapping = slot_mapping;
+    return run_q4_io<true>(p, n_layers, head_dim, dtype, (cudaStream_t)stream);
+}
+
+int qtts_kv_read_q4(const void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim, void* k, void* v,
+                    int dtype, const int64_t* k_strides, const int64_t* v_strides, int first_layer, int n_layers,
+                    const int32_t* slot_mapping, int n, qtts_stream_t stream) {
+    const int rc = q4_io_check("kv_read_q4", cache, num_blocks, num_layers, kv_heads, head_dim, k, v, dtype, k_strides,
+                               v_strides, first_layer, n_layers, slot_mapping, n);
+    if (rc || n == 0) return rc;
+    Q4IoParams p = q4_io_params(cache, num_blocks, num_layers, kv_heads, k_strides, v_strides, first_layer, n);
+    p.k_out = k;
+    p.v_out = v;
+    p.mapping = slot_mapping;
+    return run_q4_io<false>(p, n_layers, head_dim, dtype, (cudaStream_t)stream);
+}
+
+int qtts_kv_gather_q4(const void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim,
+                      const int32_t* blocks, int n_tokens, void* out, qtts_stream_t stream) {
+    const int64_t head = (int64_t)n_tokens * head_dim, kv = head * kv_heads;
+    const int64_t strides[3] = {head_dim, 2 * kv, head};
+    __half* k = reinterpret_cast<__half*>(out);
+    __half* v = k ? k + kv : nullptr;
+    const int rc = q4_io_check("kv_gather_q4", cache, num_blocks, num_layers, kv_heads, head_dim, k, v, QTTS_F16,
+                               strides, strides, 0, num_layers, blocks, n_tokens);
+    if (rc || n_tokens == 0) return rc;
+    Q4IoParams p = q4_io_params(cache, num_blocks, num_layers, kv_heads, strides, strides, 0, n_tokens);
+    p.k_out = k;
+    p.v_out = v;
+    p.blocks = blocks;
+    return run_q4_io<false>(p, num_layers, head_dim, QTTS_F16, (cudaStream_t)stream);
+}
+
+int qtts_paged_attention_window(const void* q, int R, int rows_per_stream, int num_heads, int kv_heads, int head_dim,
+                                const void* kv_pool, int layer, int num_layers, int block_size, int num_blocks,
+                                const int32_t* block_table, int num_slots, int max_blocks_per_seq,
+                                const int32_t* row_slot, const int32_t* row_ctx, int max_ctx, int window, int sinks,
+                                void* out, void* out_lo, qtts_stream_t stream) {
+    return window_attention("paged_attention_window", kWinF16, q, R, rows_per_stream, num_heads, kv_heads, head_dim,
+                            kv_pool, layer, num_layers, block_size, num_blocks, block_table, num_slots,
+                            max_blocks_per_seq, row_slot, row_ctx, max_ctx, window, sinks, out, out_lo,
+                            (cudaStream_t)stream);
+}
+
+int qtts_paged_attention_q4(const void* q, int R, int rows_per_stream, int num_heads, int kv_heads, int head_dim,
+                            const void* cache, int layer, int num_layers, int block_size, int num_blocks,
+                            const int32_t* block_table, int num_slots, int max_blocks_per_seq,
+                            const int32_t* row_slot, const int32_t* row_ctx, int max_ctx, int window, int sinks,
+                            void* out, void* out_lo, qtts_stream_t stream) {
+    return window_attention("paged_attention_q4", kWinQ4, q, R, rows_per_stream, num_heads, kv_heads, head_dim, cache,
+                            layer, num_layers, block_size, num_blocks, block_table, num_slots, max_blocks_per_seq,
+                            row_slot, row_ctx, max_ctx, window, sinks, out, out_lo, (cudaStream_t)stream);
 }
 
 int qtts_sample(const float* logits, int R, int V, int ld, int topk, const float* gumbel, int gumbel_ld, uint64_t seed,

@@ -117,6 +117,184 @@ def paged_attention_prefill(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, 
     return out
 
 
+# --------------------------------------------------------------------------- 4-bit KV cache, windowed attention
+_DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
+
+
+def _same_device(*ts) -> torch.device:
+    _need_cuda(*ts)
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev
+
+
+class _on:
+    """Makes ``dev`` current while a kernel is launched (a no-op when it already is)."""
+
+    def __init__(self, dev: torch.device):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _need_i32(name: str, t: torch.Tensor, ndim: int):
+    if t.dtype != torch.int32 or t.dim() != ndim or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor of {ndim} dimension(s)")
+
+
+def _q4_dims(cache: torch.Tensor):
+    """(blocks, layers, kv heads, head_dim) of a 4-bit pool."""
+    if cache.dtype != torch.uint8 or cache.dim() != 5 or cache.shape[2] != 2 or not cache.is_contiguous():
+        raise ValueError("q4 cache: a contiguous uint8 tensor [blocks, layers, 2, kv_heads, 9 * head_dim]")
+    nb, L, _, H, chunk = cache.shape
+    if chunk not in (9 * 64, 9 * 128):
+        raise ValueError(f"q4 cache: {chunk} bytes per chunk (head_dim 64 has 576, 128 has 1152)")
+    return nb, L, H, chunk // 9
+
+
+def _q4_rows(name: str, t: torch.Tensor, n: int, layers: Optional[int], H: int, D: int):
+    """``[n, layers, H, D]`` view of K or V rows and its (token, layer, head) strides."""
+    if t.dim() == 3:
+        t = t.unsqueeze(1)
+    if t.dim() != 4 or t.shape[0] != n or t.shape[2:] != (H, D) or (layers is not None and t.shape[1] != layers):
+        raise ValueError(f"{name}: rows [{n}, {'layers' if layers is None else layers}, {H}, {D}], got {tuple(t.shape)}")
+    if t.dtype not in _DT:
+        raise ValueError(f"{name}: float16, bfloat16 or float32, got {t.dtype}")
+    if t.stride(3) != 1:
+        raise ValueError(f"{name}: channels must be contiguous")
+    return t, (C.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+
+
+def kv_write_q4(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
+                layer: int = 0) -> None:
+    """Quantise K/V rows ``[n, Hkv, D]`` (one layer) or ``[n, layers, Hkv, D]`` (from ``layer`` on), fp16,
+    bf16 or fp32 with any token, layer and head strides, into the positions ``slot_mapping [n]`` (block
+    * 16 + offset, int32, distinct; negative ones are skipped) of a 4-bit pool."""
+    dev = _same_device(cache, k, v, slot_mapping)
+    nb, L, H, D = _q4_dims(cache)
+    _need_i32("slot_mapping", slot_mapping, 1)
+    n = slot_mapping.numel()
+    k, ks = _q4_rows("k", k, n, None, H, D)
+    v, vs = _q4_rows("v", v, n, k.shape[1], H, D)
+    if k.dtype != v.dtype:
+        raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
+    with _on(dev):
+        rc = _lib.load().qtts_kv_write_q4(cache.data_ptr(), nb, L, H, D, k.data_ptr(), v.data_ptr(), _DT[k.dtype], ks,
+                                          vs, layer, k.shape[1], slot_mapping.data_ptr(), n, _lib.stream_ptr())
+    _lib.check(rc, "kv_write_q4")
+
+
+def kv_read_q4(cache: torch.Tensor, slot_mapping: torch.Tensor, layer: int = 0, n_layers: int = 1,
+               dtype: torch.dtype = torch.float16, k: Optional[torch.Tensor] = None,
+               v: Optional[torch.Tensor] = None):
+    """What the positions ``slot_mapping [n]`` of a 4-bit pool hold: ``(k, v)``, each ``[n, n_layers, Hkv,
+    D]`` in ``dtype`` (or written to the given ``k``, ``v``); positions outside the pool read as zeros."""
+    dev = _same_device(cache, slot_mapping, k, v)
+    nb, L, H, D = _q4_dims(cache)
+    _need_i32("slot_mapping", slot_mapping, 1)
+    n = slot_mapping.numel()
+    if dtype not in _DT:
+        raise ValueError(f"kv_read_q4: float16, bfloat16 or float32, got {dtype}")
+    if n_layers < 1 or layer < 0 or layer + n_layers > L:
+        raise ValueError(f"kv_read_q4: layers [{layer}, +{n_layers}) of {L}")
+    if k is None:
+        k = torch.empty(n, n_layers, H, D, device=dev, dtype=dtype)
+    if v is None:
+        v = torch.empty(n, n_layers, H, D, device=dev, dtype=k.dtype)
+    kr, ks = _q4_rows("k", k, n, n_layers, H, D)
+    vr, vs = _q4_rows("v", v, n, n_layers, H, D)
+    if kr.dtype != vr.dtype:
+        raise ValueError(f"k is {kr.dtype}, v is {vr.dtype}")
+    with _on(dev):
+        rc = _lib.load().qtts_kv_read_q4(cache.data_ptr(), nb, L, H, D, kr.data_ptr(), vr.data_ptr(), _DT[kr.dtype],
+                                         ks, vs, layer, n_layers, slot_mapping.data_ptr(), n, _lib.stream_ptr())
+    _lib.check(rc, "kv_read_q4")
+    return k, v
+
+
+def kv_gather_q4(cache: torch.Tensor, blocks: torch.Tensor, n_tokens: int,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The first ``n_tokens`` tokens of a block list (a block-table row, a prefix entry's ids) of a 4-bit
+    pool, all layers: fp16 ``[2 L, Hkv, n_tokens, D]``, as :meth:`Sched.gather` of the fp16 pool."""
+    dev = _same_device(cache, blocks, out)
+    nb, L, H, D = _q4_dims(cache)
+    _need_i32("blocks", blocks, 1)
+    if n_tokens < 0 or n_tokens > 16 * blocks.numel():
+        raise ValueError(f"kv_gather_q4: {n_tokens} tokens of {blocks.numel()} blocks")
+    if out is None:
+        out = torch.empty(2 * L, H, n_tokens, D, device=dev, dtype=torch.float16)
+    elif out.dtype != torch.float16 or out.shape != (2 * L, H, n_tokens, D) or not out.is_contiguous():
+        raise ValueError(f"kv_gather_q4: out must be contiguous fp16 [{2 * L}, {H}, {n_tokens}, {D}]")
+    with _on(dev):
+        rc = _lib.load().qtts_kv_gather_q4(cache.data_ptr(), nb, L, H, D, blocks.data_ptr(), n_tokens, out.data_ptr(),
+                                           _lib.stream_ptr())
+    _lib.check(rc, "kv_gather_q4")
+    return out
+
+
+def _window_attention(what: str, q, kv, dims, layer, block_table, row_slot, row_ctx, max_ctx, window, sinks,
+                      rows_per_stream, out, out_lo):
+    dev = _same_device(q, kv, block_table, row_slot, row_ctx, out, out_lo)
+    nb, L, H, D = dims
+    if q.dim() != 3 or q.dtype != torch.float32 or not q.is_contiguous() or q.shape[2] != D:
+        raise ValueError(f"{what}: q must be contiguous float32 [rows, heads, {D}]")
+    R, Hq, _ = q.shape
+    _need_i32("block_table", block_table, 2)
+    _need_i32("row_slot", row_slot, 1)
+    _need_i32("row_ctx", row_ctx, 1)
+    if row_slot.numel() != R or row_ctx.numel() != R:
+        raise ValueError(f"{what}: {R} query rows, {row_slot.numel()} slots and {row_ctx.numel()} contexts")
+    if out is None:
+        out = torch.empty(R, Hq * D, device=dev, dtype=torch.bfloat16)
+    for o in (out, out_lo):
+        if o is not None and (o.dtype != torch.bfloat16 or o.numel() != R * Hq * D or not o.is_contiguous()):
+            raise ValueError(f"{what}: out and out_lo must be contiguous bfloat16 [{R}, {Hq * D}]")
+    with _on(dev):
+        rc = getattr(_lib.load(), "qtts_" + what)(q.data_ptr(), R, rows_per_stream, Hq, H, D, kv.data_ptr(), layer, L,
+                                                  16, nb, block_table.data_ptr(), block_table.shape[0],
+                                                  block_table.shape[1], row_slot.data_ptr(), row_ctx.data_ptr(),
+                                                  max_ctx, window, sinks, out.data_ptr(), _lib.ptr(out_lo),
+                                                  _lib.stream_ptr())
+    _lib.check(rc, what)
+    return out
+
+
+def paged_attention_window(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, block_table: torch.Tensor,
+                           row_slot: torch.Tensor, row_ctx: torch.Tensor, max_ctx: int, window: int, sinks: int = 0,
+                           rows_per_stream: int = 1, out: Optional[torch.Tensor] = None,
+                           out_lo: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_attention` under a sliding window: a row of context ``c`` sees key ``j < c`` when ``j >=
+    c - window`` or ``j < sinks`` (``window`` 0: every key).  ``q [R, Hq, D]`` fp32 over ``kv_pool [blocks,
+    L, 2, Hkv, 16, D]`` fp16, ``D`` 64 or 128, any whole ``Hq / Hkv``; rows without a visible key get
+    zeros.  ``rows_per_stream`` > 1: the rows are streams of that many consecutive query tokens (a
+    prompt chunk), which share the blocks they read.  Returns bf16 ``[R, Hq * D]`` (``out_lo``: its bf16
+    residual)."""
+    if kv_pool.dtype != torch.float16 or kv_pool.dim() != 6 or kv_pool.shape[2] != 2 or kv_pool.shape[4] != 16 \
+            or not kv_pool.is_contiguous():
+        raise ValueError("paged_attention_window: a contiguous float16 pool [blocks, layers, 2, kv_heads, 16, head_dim]")
+    nb, L, _, H, _, D = kv_pool.shape
+    return _window_attention("paged_attention_window", q, kv_pool, (nb, L, H, D), layer, block_table, row_slot, row_ctx,
+                             max_ctx, window, sinks, rows_per_stream, out, out_lo)
+
+
+def paged_attention_q4(q: torch.Tensor, cache: torch.Tensor, layer: int, block_table: torch.Tensor,
+                       row_slot: torch.Tensor, row_ctx: torch.Tensor, max_ctx: int, window: int = 0, sinks: int = 0,
+                       rows_per_stream: int = 1, out: Optional[torch.Tensor] = None,
+                       out_lo: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_attention_window` over a 4-bit pool ``cache [blocks, L, 2, Hkv, 9 D]`` (uint8, written by
+    :func:`kv_write_q4`); every key is visible by default."""
+    return _window_attention("paged_attention_q4", q, cache, _q4_dims(cache), layer, block_table, row_slot, row_ctx,
+                             max_ctx, window, sinks, rows_per_stream, out, out_lo)
+
+
 def sample(logits: torch.Tensor, topk: int, gumbel: Optional[torch.Tensor] = None, temperature=None, penalty=None,
            counts: Optional[torch.Tensor] = None, eos_id: int = -1, seed: int = 0,
            noise_key: Optional[torch.Tensor] = None, step: int = 0, tok_out: Optional[torch.Tensor] = None,
@@ -211,7 +389,9 @@ class Sched:
         _lib.check(self.lib.qtts_sched_release(C.byref(self.pool.state), slot, _lib.stream_ptr()), "sched_release")
 
     def scatter(self, rows: torch.Tensor, mapping: torch.Tensor):
-        """rows ``[n, L*2, Hkv, D]`` bf16 into the pool."""
+        """rows ``[n, L*2, Hkv, D]`` fp16 into the pool (quantised when it is a 4-bit one)."""
+        if self.pool.kv.dtype == torch.uint8:
+            return kv_write_q4(self.pool.kv, rows[:, 0::2], rows[:, 1::2], mapping)
         L2, Hkv, D = rows.shape[1:]
         rc = self.lib.qtts_kv_scatter(self.pool.kv.data_ptr(), C.byref(self.pool.state), L2 // 2, Hkv, D,
                                       rows.data_ptr(), mapping.data_ptr(), rows.shape[0], _lib.stream_ptr())
@@ -219,6 +399,10 @@ class Sched:
 
     def gather(self, slot: int, n: int) -> torch.Tensor:
         kv = self.pool.kv
+        if kv.dtype == torch.uint8:
+            if not 0 <= slot < self.pool.block_table.shape[0]:
+                raise ValueError(f"kv_gather: slot {slot}")
+            return kv_gather_q4(kv, self.pool.block_table[slot], n)
         L, Hkv, D = kv.shape[1], kv.shape[3], kv.shape[5]
         out = torch.empty(2 * L, Hkv, n, D, device=kv.device, dtype=torch.float16)
         rc = self.lib.qtts_kv_gather(kv.data_ptr(), C.byref(self.pool.state), L, Hkv, D, slot, n, out.data_ptr(),

@@ -45,9 +45,16 @@ def _interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 class PagedPoolTensors:
-    """Device arrays of the paged allocator plus the KV block storage."""
+    """Device arrays of the paged allocator plus the KV block storage.
 
-    def __init__(self, cfg: EngineConfig, device):
+    ``kv_format`` "fp16" is the pool the engine runs on.  "q4" holds the same blocks in 4.5 bits an
+    element (``ops.kv_write_q4`` / ``kv_read_q4`` / ``paged_attention_q4``; layout in
+    ``qtts_b200.h``) as bytes ``[num_blocks][L][2][Hkv][9 D]``; the allocator, block sharing and
+    copy-on-write (``ops.Sched``) work on either."""
+
+    def __init__(self, cfg: EngineConfig, device, kv_format: str = "fp16"):
+        if kv_format not in ("fp16", "q4"):
+            raise ValueError(f"kv_format {kv_format!r}: fp16 or q4")
         t, p = cfg.talker, cfg.pool
         i32 = dict(device=device, dtype=torch.int32)
         self.free_stack = torch.empty(p.num_blocks, **i32)
@@ -58,9 +65,16 @@ class PagedPoolTensors:
         self.position_offset = torch.empty(p.max_slots, **i32)
         # zero-filled: attention kernels multiply V rows past a sequence's last key by P = 0, so the
         # pool must never hold a non-finite value (it only ever receives written K/V after this)
-        self.kv = torch.zeros(p.num_blocks, t.num_layers, 2, t.kv_heads, p.block_size, t.head_dim,
-                              device=device, dtype=torch.float16)
-        self.block_elems = t.num_layers * 2 * t.kv_heads * p.block_size * t.head_dim
+        if kv_format == "q4":
+            if t.head_dim not in (64, 128) or p.block_size != 16:
+                raise ValueError("a q4 pool needs head_dim 64 or 128 and 16-token blocks")
+            self.kv = torch.zeros(p.num_blocks, t.num_layers, 2, t.kv_heads, 9 * t.head_dim, device=device,
+                                  dtype=torch.uint8)
+        else:
+            self.kv = torch.zeros(p.num_blocks, t.num_layers, 2, t.kv_heads, p.block_size, t.head_dim,
+                                  device=device, dtype=torch.float16)
+        # 2-byte units of one block, what a copy-on-write moves
+        self.block_elems = self.kv[0].numel() * self.kv.element_size() // 2
         self.state = _lib.PagedState(
             self.free_stack.data_ptr(), self.free_top.data_ptr(), self.refcount.data_ptr(),
             self.block_table.data_ptr(), self.seq_len.data_ptr(), self.position_offset.data_ptr(),
