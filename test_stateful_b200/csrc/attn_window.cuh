@@ -7,12 +7,17 @@
 // Row kernel.  One warp walks 16-token blocks, copied ahead of use into a ring of its own in shared
 // memory (cp.async, 16 bytes a lane).  The tensor work is mma.sync m16n8k16 with the keys on the M
 // side and (query, head) slots on the N side:
-//     S^T[16 tokens][8]   += K[16][16 channels] . Q^T       D/16 instructions a block
-//     O^T[16 channels][8] += V^T[16][16 tokens] . P^T       D/16 instructions a block
-// Four slots fill the eight columns: columns 0-3 carry the operand's high half, 4-7 what rounding
-// took from it, so that q and the probabilities keep 16 bits or more at no extra instructions;
-// lanes t and t ^ 2 of a quad hold the two halves of the same scores.  movmatrix turns the
+//     S^T[16 tokens][8]   += K[16][16 channels] . Q^T       2 x D/16 instructions a block
+//     O^T[16 channels][8] += V^T[16][16 tokens] . P^T       D/16 or 2 x D/16 instructions a block
+// Both operands on the N side are pairs of 16-bit halves (what rounding took from the first is the
+// second), so that q and the probabilities keep 16 bits or more.  movmatrix turns the
 // probabilities from S^T's accumulator layout into the operand layout.
+// Decode tiles fill few of the eight columns (two query heads a KV head: two).  There the columns
+// are shared by KB = 8 / SL blocks of SL slots: q stands in every group of columns, so that each
+// lane of a quad finds the scores of one block in its registers and the softmax of KB blocks runs
+// at once, a block to a lane; for P V each block takes its own group's columns of P and the opposite
+// group's hold the second halves, the rest zero.  The column groups of O add up at the end.  (64
+// streams x 4096 keys, 4 bits: 388 instructions a block with one block at a time.)
 //
 // 4-bit pool: a nibble masked out of a code word IS a small fp16 or bf16 number (a subnormal:
 // nibble << 0 = code * 2^-24 or 2^-133, nibble << 4 = 16 times that), so that no conversion is
@@ -22,6 +27,8 @@
 // the channels 64 w + 16 t .. + 15, of V tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 the channels
 // 64 w + 8 g .. + 7.
 #pragma once
+
+#include <type_traits>
 
 #include "attention.cuh"
 #include "kv_q4.cuh"
@@ -43,6 +50,7 @@ struct WinParams {
     int qt, tiles;          // queries per tile, tiles per stream
     int layer, num_layers, num_blocks, num_slots, mbps;
     int max_ctx, window, sinks;
+    uint32_t block_bytes, v_offset;  // of one pool block; from a K chunk to its V chunk
     float scale_log2;       // log2(e) / sqrt(D)
 };
 
@@ -53,6 +61,14 @@ __device__ __forceinline__ void mma_16816_bf16(float (&d)[4], const uint32_t (&a
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// D = A B, the first of a chain
+__device__ __forceinline__ void mma_16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // transpose of an 8 x 8 matrix of 16-bit elements held as two per lane
@@ -131,20 +147,22 @@ struct WinStage {
 constexpr float kPScale = 1.2676506002282294e30f;  // 2^100
 constexpr float kPUnscale = 8589934592.f;          // 2^133 / 2^100
 
-// NB: column groups of four slots.  W warps per CTA, ST stages per warp.
-template <int FMT, int D, int NB, int W, int ST>
+// SL slots a tile, W warps per CTA, two stages of KB blocks per warp.
+template <int FMT, int D, int SL, int W>
 __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinParams p) {
     using G = WinStage<FMT, D>;
-    constexpr int NW = G::NW, MT = D / 16, SL = 4 * NB;
+    constexpr int NW = G::NW, MT = D / 16, KB = 8 / SL;
+    constexpr int STAGE = KB * G::BYTES;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_ml[W][SL][2];
     __shared__ float s_part[SL][2];  // the CTA's (max, sum) per slot
-    static_assert(SL * D * 4 <= ST * G::BYTES, "a warp's partial output replaces its ring");
+    static_assert(SL * D * 4 <= 2 * STAGE, "a warp's partial output replaces its ring");
 
     griddep_wait();
     griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
+    const int kb = 2 * t / SL;  // the block of an iteration whose scores this lane holds
     uint32_t splits;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
     const uint32_t rank = cluster_ctarank();
@@ -159,79 +177,76 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
     const int row0 = stream * p.S + q0;
     const int slots = nq * heads;
 
-    // contexts: this lane's slots, and the tile's extremes over rows that see anything
+    // contexts: this lane's score columns, and the tile's extremes over rows that see anything
     const int limit = min(p.max_ctx, p.mbps * 16);
     const int window = p.window > 0 ? p.window : 0x7fffffff;
     const int slot = __ldg(p.row_slot + row0);
     const bool slot_ok = slot >= 0 && slot < p.num_slots;
-    int ctx[NB][2];
+    int ctx[2];
     int cmax = 0, cmin = 0x7fffffff;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int e = 0; e < 2; ++e) {
+        const int s = (2 * t + e) % SL;
+        ctx[e] = s < slots && slot_ok ? min(max(__ldg(p.row_ctx + row0 + s / heads), 0), limit) : 0;
+        cmax = max(cmax, ctx[e]);
+        if (ctx[e] > 0) cmin = min(cmin, ctx[e]);
+    }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int s = 4 * b + 2 * (t & 1) + e;
-            ctx[b][e] = s < slots && slot_ok ? min(max(__ldg(p.row_ctx + row0 + s / heads), 0), limit) : 0;
-            cmax = max(cmax, ctx[b][e]);
-            if (ctx[b][e] > 0) cmin = min(cmin, ctx[b][e]);
-        }
-    cmax = max(cmax, __shfl_xor_sync(0xffffffffu, cmax, 1));
-    cmin = min(cmin, __shfl_xor_sync(0xffffffffu, cmin, 1));
+    for (int x = 1; x < 4; x <<= 1) {
+        cmax = max(cmax, __shfl_xor_sync(0xffffffffu, cmax, x));
+        cmin = min(cmin, __shfl_xor_sync(0xffffffffu, cmin, x));
+    }
     if (!slot_ok && threadIdx.x == 0) record_error(DEV_ERR_ATTN_BOUNDS);
     // blocks that hold a visible key: the sinks', then from the earliest window's start
     const int nb_end = (cmax + 15) >> 4;
     const int nb_sink = min((min(p.sinks, cmax) + 15) >> 4, nb_end);
     const int first = max(nb_sink, cmax > 0 ? max(0, cmin - window) >> 4 : 0);
+    const int past_sinks = first - nb_sink;  // what the blocks after the sinks' skip
     const int nb = nb_sink + max(0, nb_end - first);
-    const int stride = (int)splits * W;
-    const int i0 = (int)rank * W + warp;
-    const int mine = i0 < nb ? (nb - i0 + stride - 1) / stride : 0;
-    auto block_no = [&](int n) {  // the warp's n-th block
-        const int i = i0 + n * stride;
-        return i < nb_sink ? i : first + (i - nb_sink);
-    };
+    // this warp's share of them: [i0, i0 + mine)
+    const int workers = (int)splits * W, me = (int)rank * W + warp;
+    const int even = nb / workers, rest = nb % workers;
+    const int i0 = me * even + min(me, rest), mine = even + (me < rest);
 
-    // ids of the warp's next 32 blocks, one per lane; an id outside the pool hides its keys
+    // ids of the warp's next 32 blocks, one per lane
     const int32_t* table = p.block_table + (size_t)(slot_ok ? slot : 0) * p.mbps;
-    const size_t block_stride = (size_t)p.num_layers * 2 * p.kv_heads * G::CHUNK;
     const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::CHUNK;
-    const size_t v_off = (size_t)p.kv_heads * G::CHUNK;
-    const uint32_t ring = smem_u32(smem) + warp * ST * G::BYTES;
-    int ids = -1;
-    auto issue = [&](int n) {  // copy block n into its stage; every lane commits a group, full or empty
+    const uint32_t ring = smem_u32(smem) + warp * 2 * STAGE;
+    int ids = 0;
+    bool bad_id = false;  // an id outside the pool came up: its keys are hidden
+    auto table_id = [&](int n) {  // of the warp's block n
+        const int i = i0 + n;
+        return __ldg(table + (i < nb_sink ? i : i + past_sinks));
+    };
+    auto issue = [&](int n, uint32_t stage) {  // copy blocks n .. n + KB - 1; every lane commits a group, full or empty
         if (n < mine) {
             if ((n & 31) == 0) {
-                ids = -1;
-                if (n + lane < mine) {
-                    const int b = __ldg(table + block_no(n + lane));
-                    if (b >= 0 && b < p.num_blocks) ids = b;
-                    else record_error(DEV_ERR_ATTN_BOUNDS);
+                ids = n + lane < mine ? table_id(n + lane) : 0;
+                const bool out = ids < 0 || ids >= p.num_blocks;
+                if (__any_sync(0xffffffffu, out)) bad_id = true;
+                if (out) {
+                    record_error(DEV_ERR_ATTN_BOUNDS);
+                    ids = 0;
                 }
             }
-            const int id = __shfl_sync(0xffffffffu, ids, n & 31);
-            if (id >= 0) {
-                const uint8_t* c = base + (size_t)id * block_stride;
-                G::copy(ring + (n % ST) * G::BYTES, c, c + v_off, lane);
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                if (k > 0 && n + k >= mine) break;
+                const uint8_t* c = base + (uint64_t)(uint32_t)__shfl_sync(0xffffffffu, ids, (n & 31) + k) * p.block_bytes;
+                G::copy(stage + k * G::BYTES, c, c + p.v_offset, lane);
             }
-            cp_async_commit();
-            return id >= 0;
         }
         cp_async_commit();
-        return false;
     };
-    uint32_t present = 0;  // bit n % 32: block n is in the pool
-#pragma unroll
-    for (int n = 0; n < ST - 1; ++n)
-        if (issue(n)) present |= 1u << n;
+    issue(0, ring);
 
     // Q^T operand.  Each slot's q is scaled by a power of two that brings its largest channel to
     // [2^11, 2^12), so that fp16 halves hold it whatever its size; the upper nibbles' channels take
-    // 1/16.  Lane (g, t) holds column g: slot g % 4 of each column group, high (g < 4) or low half.
-    uint32_t qb[NB][MT][2];
-    float sf[NB][2], qsum[NB][NW][2];  // of this lane's score columns: accumulator -> log2 units, sum of q
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int s = 4 * b + (g & 3);
+    // 1/16.  Lane (g, t) holds column g: slot g % SL.
+    uint32_t qb[MT][2], ql[MT][2];
+    float sf[2], qsum[NW][2];  // of this lane's score columns: accumulator -> log2 units, sum of q
+    {
+        const int s = g % SL;
         const bool valid = s < slots;
         const float* qr = p.q + ((size_t)(row0 + (valid ? s / heads : 0)) * p.num_heads + kvh * p.group + h0 +
                                  (valid ? s % heads : 0)) * D;
@@ -264,17 +279,13 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
         float f = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
         if constexpr (FMT == kWinQ4) f *= 16777216.f;  // 2^24
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {  // column 2 t + e belongs to lane (2 (t % 2) + e, any)
-            const int src = 4 * (2 * (t & 1) + e);
-            sf[b][e] = __shfl_sync(0xffffffffu, f, src);
-        }
+        for (int e = 0; e < 2; ++e) sf[e] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + e));
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 1);
             sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 2);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                qsum[b][w][e] = __shfl_sync(0xffffffffu, sum[w], 4 * (2 * (t & 1) + e)) * p.scale_log2;
+            for (int e = 0; e < 2; ++e) qsum[w][e] = __shfl_sync(0xffffffffu, sum[w], 4 * (2 * t + e)) * p.scale_log2;
 #pragma unroll
             for (int s4 = 0; s4 < 4; ++s4) {
                 float x[4];
@@ -286,133 +297,111 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
 #pragma unroll
                     for (int c = 0; c < 4; ++c) x[c] = v[w][4 * s4 + c] * up;
                 }
-                uint32_t hi, lo;
-                split_h2(x[0], x[1], hi, lo);
-                qb[b][4 * w + s4][0] = g < 4 ? hi : lo;
-                split_h2(x[2], x[3], hi, lo);
-                qb[b][4 * w + s4][1] = g < 4 ? hi : lo;
+                split_h2(x[0], x[1], qb[4 * w + s4][0], ql[4 * w + s4][0]);
+                split_h2(x[2], x[3], qb[4 * w + s4][1], ql[4 * w + s4][1]);
             }
         }
     }
 
-    float o[NB][MT][4];  // FMT q4: row tile 4 w + k holds channels 64 w + 8 g + 2 k (c 0, 1) and + 1 (c 2, 3)
-    float zacc[NB][NW][2], m[NB][2], l[NB][2];
+    float o[MT][4];  // FMT q4: row tile 4 w + k holds channels 64 w + 8 g + 2 k (c 0, 1) and + 1 (c 2, 3)
+    float zacc[NW][2], l[2] = {0.f, 0.f};
+    // running maximum of the two columns' slots, and what probabilities are relative to (0 until a key is seen)
+    float m[2] = {-INFINITY, -INFINITY}, mu[2] = {0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
+    for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            m[b][e] = -INFINITY;
-            l[b][e] = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) zacc[b][w][e] = 0.f;
-        }
-    }
-    const uint32_t lo_mask = t < 2 ? 0u : 0xffff0000u;  // lanes of the low columns keep x - high(x)
+    for (int w = 0; w < NW; ++w) zacc[w][0] = zacc[w][1] = 0.f;
 
-    for (int n = 0; n < mine; ++n) {
-        cp_async_wait<ST - 2>();
-        __syncwarp();  // every lane's copies of block n are there, and every lane is done with block n - 1
-        {
-            const bool in = issue(n + ST - 1);
-            const uint32_t bit = 1u << ((n + ST - 1) & 31);
-            present = in ? present | bit : present & ~bit;
-        }
-        const uint32_t ks = ring + (n % ST) * G::BYTES, vs = ks + G::CHUNK;
-        if (!((present >> (n & 31)) & 1)) continue;
-        const int j0 = block_no(n) * 16;
+    // one iteration's blocks (n_here of them) in a stage; MASKED: some row does not see all of them.
+    // j0: first token of this lane's block; present: it is there and in the pool
+    auto blocks = [&](auto masked, const uint32_t stage, const int n_here, const int j0, const bool present) {
+        constexpr bool MASKED = decltype(masked)::value;
+        auto sees = [&](int i) {  // score i: token g + 8 (i / 2) of block kb, column 2 t + i % 2
+            const int j = j0 + g + 8 * (i >> 1), c = ctx[i & 1];
+            return present && j < c && (j >= c - window || j < p.sinks);
+        };
+        const uint32_t my_stage = stage + kb * G::BYTES;
 
-        // S^T
-        float s[NB][4];
+        // S^T, relative to mu
+        float s[4];
         if constexpr (FMT == kWinQ4) {
-            uint32_t kg[2 * NW], kh[2 * NW];  // tokens g, g + 8: word 2 w' + ... as stored (e * NW + w)
-            const int row = g * (D / 2) + t * 8 * NW;
-            const int sw = D == 128 ? row ^ (((g >> 1) & 3) << 5) : row;
-            lds_words(kg, ks + sw);
-            lds_words(kh, ks + sw + 8 * (D / 2));
-            float acc[NB][NW][4];
+            float acc[NW][4];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
+            for (int k = 0; k < KB; ++k) {
+                if (MASKED && k > 0 && k >= n_here) break;
+                const uint32_t ks = stage + k * G::BYTES;
+                uint32_t kg[2 * NW], kh[2 * NW];  // tokens g, g + 8
+                const int row = g * (D / 2) + t * 8 * NW;
+                const int sw = D == 128 ? row ^ (((g >> 1) & 3) << 5) : row;
+                lds_words(kg, ks + sw);
+                lds_words(kh, ks + sw + 8 * (D / 2));
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b][w][0] = acc[b][w][1] = acc[b][w][2] = acc[b][w][3] = 0.f;
+                for (int w = 0; w < NW; ++w) {
+                    float d[4];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t x = kg[e * NW + w], y = kh[e * NW + w];
-                    const uint32_t a1[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
-                    const uint32_t a2[4] = {(x >> 8) & 0x000f000fu, (y >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u,
-                                            (y >> 8) & 0x00f000f0u};
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        mma_16816(acc[b][w], a1, qb[b][4 * w + 2 * e][0], qb[b][4 * w + 2 * e][1]);
-                        mma_16816(acc[b][w], a2, qb[b][4 * w + 2 * e + 1][0], qb[b][4 * w + 2 * e + 1][1]);
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t x = kg[e * NW + w], y = kh[e * NW + w];
+                        const uint32_t a1[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+                        const uint32_t a2[4] = {(x >> 8) & 0x000f000fu, (y >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u,
+                                                (y >> 8) & 0x00f000f0u};
+                        const int q1 = 4 * w + 2 * e, q2 = q1 + 1;
+                        if (e == 0) mma_16816_zero(d, a1, qb[q1][0], qb[q1][1]);
+                        else mma_16816(d, a1, qb[q1][0], qb[q1][1]);
+                        mma_16816(d, a2, qb[q2][0], qb[q2][1]);
+                        mma_16816(d, a1, ql[q1][0], ql[q1][1]);
+                        mma_16816(d, a2, ql[q2][0], ql[q2][1]);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (k == 0 || kb == k) acc[w][i] = d[i];
                 }
             }
             float2 kp[NW][2];
 #pragma unroll
             for (int w = 0; w < NW; ++w)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) kp[w][h] = lds_half2(ks + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
+                for (int h = 0; h < 2; ++h)
+                    kp[w][h] = lds_half2(my_stage + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float d = acc[b][0][i] * kp[0][i >> 1].x, z = qsum[b][0][i & 1] * kp[0][i >> 1].y;
-                    if constexpr (NW == 2) {
-                        d = fmaf(acc[b][1][i], kp[1][i >> 1].x, d);
-                        z = fmaf(qsum[b][1][i & 1], kp[1][i >> 1].y, z);
-                    }
-                    d += __shfl_xor_sync(0xffffffffu, d, 2);
-                    s[b][i] = fmaf(d, sf[b][i & 1], z);
+            for (int i = 0; i < 4; ++i) {
+                float d = acc[0][i] * kp[0][i >> 1].x;
+                float z = fmaf(qsum[0][i & 1], kp[0][i >> 1].y, -mu[i & 1]);
+                if constexpr (NW == 2) {
+                    d = fmaf(acc[1][i], kp[1][i >> 1].x, d);
+                    z = fmaf(qsum[1][i & 1], kp[1][i >> 1].y, z);
                 }
+                s[i] = fmaf(d, sf[i & 1], z);
+            }
         } else {
-            float acc[NB][2][4];  // two chains
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[b][0][i] = acc[b][1][i] = 0.f;
+            float acc[2][4];  // two chains
             const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 uint32_t a[4];
                 const int c = 2 * i + (lane >> 4);
-                ldsm_x4(ks + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) mma_16816(acc[b][i & 1], a, qb[b][i][0], qb[b][i][1]);
+                ldsm_x4(stage + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
+                if (i < 2) mma_16816_zero(acc[i & 1], a, qb[i][0], qb[i][1]);
+                else mma_16816(acc[i & 1], a, qb[i][0], qb[i][1]);
+                mma_16816(acc[i & 1], a, ql[i][0], ql[i][1]);
             }
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float d = acc[b][0][i] + acc[b][1][i];
-                    d += __shfl_xor_sync(0xffffffffu, d, 2);
-                    s[b][i] = d * sf[b][i & 1];
-                }
+            for (int i = 0; i < 4; ++i) s[i] = fmaf(acc[0][i] + acc[1][i], sf[i & 1], -mu[i & 1]);
         }
 
-        // the mask, where the block is not visible to every row as a whole
-        const bool whole = j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks);
-        auto sees = [&](int b, int i) {  // row of score i: token g + 8 (i / 2), column 2 t + i % 2
-            const int j = j0 + g + 8 * (i >> 1), c = ctx[b][i & 1];
-            return j < c && (j >= c - window || j < p.sinks);
-        };
-        if (!whole) {
+        if constexpr (MASKED) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!sees(b, i)) s[b][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+                if (!sees(i)) s[i] = -INFINITY;
             if constexpr (FMT == kWinF16) {
                 // a key that some row does not see must not reach it through 0 * V: what is not
                 // finite in such a row of V is set to zero, and the rows that do see it become NaN
                 const int r = lane >> 1, j = j0 + r;
-                const bool all = j < cmin && (j >= cmax - window || j < p.sinks);
+                const bool all = present && j < cmin && (j >= cmax - window || j < p.sinks);
                 bool bad = false;
                 if (!all) {
 #pragma unroll
                     for (int c = 0; c < D / 16; ++c) {
-                        const uint32_t at = vs + (r * (D / 8) + (((lane & 1) * (D / 16) + c) ^ (r & 7))) * 16;
+                        const uint32_t at = stage + G::CHUNK + (r * (D / 8) + (((lane & 1) * (D / 16) + c) ^ (r & 7))) * 16;
                         uint32_t u[4];
                         lds_words(u, at);
                         bool here = false;
@@ -432,11 +421,8 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
                 if (rows) {
                     __syncwarp();
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (((rows >> (2 * (g + 8 * (i >> 1)))) & 3) && sees(b, i))
-                                l[b][i & 1] = __int_as_float(0x7fffffff);
+                    for (int i = 0; i < 4; ++i)
+                        if (((rows >> (2 * (g + 8 * (i >> 1)))) & 3) && sees(i)) l[i & 1] = __int_as_float(0x7fffffff);
                 }
             }
         }
@@ -445,138 +431,184 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
         // 8, so that probabilities stay below 2^8
         bool grow = false;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[b][e], s[b][2 + e]) > m[b][e] + 8.f;
+        for (int e = 0; e < 2; ++e) grow |= fmaxf(s[e], s[2 + e]) > (m[e] == -INFINITY ? -INFINITY : 8.f);
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int e = 0; e < 2; ++e) {
+                float mn = fmaxf(s[e], s[2 + e]) + mu[e];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float mn = fmaxf(m[b][e], fmaxf(s[b][e], s[b][2 + e]));
+                for (int x = SL / 2; x < 32; x <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+                mn = fmaxf(mn, m[e]);
+                const float corr = mn == -INFINITY ? 1.f : ex2_approx(m[e] - mn);
+                const float to = mn == -INFINITY ? 0.f : mn;
+                s[e] += mu[e] - to;
+                s[2 + e] += mu[e] - to;
+                m[e] = mn;
+                mu[e] = to;
+                l[e] *= corr;
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
-                    const float corr = mn == -INFINITY ? 1.f : ex2_approx(m[b][e] - mn);
-                    m[b][e] = mn;
-                    l[b][e] *= corr;
+                for (int w = 0; w < NW; ++w) zacc[w][e] *= corr;
 #pragma unroll
-                    for (int w = 0; w < NW; ++w) zacc[b][w][e] *= corr;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        o[b][i][e] *= corr;
-                        o[b][i][2 + e] *= corr;
-                    }
+                for (int i = 0; i < MT; ++i) {
+                    o[i][e] *= corr;
+                    o[i][2 + e] *= corr;
                 }
-        }
-        float pr[NB][4];
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float mu = m[b][i & 1] == -INFINITY ? 0.f : m[b][i & 1];
-                pr[b][i] = ex2_approx(s[b][i] - mu);
-                l[b][i & 1] += pr[b][i];
             }
+        }
+        float pr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            pr[i] = ex2_approx(s[i]);
+            l[i & 1] += pr[i];
+        }
 
         // O^T += V^T P^T
         if constexpr (FMT == kWinQ4) {
-            uint32_t v[4][NW];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 2 * t + (i & 1) + 8 * (i >> 1), at = r * (D / 2) + g * 4 * NW;
-                lds_words(v[i], vs + (D == 128 ? at ^ (t << 5) : at));
-            }
+            uint32_t ph[NW][2], pl[NW][2];  // P^T operands of the KB blocks: column g belongs to block g / SL
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
-                uint32_t pb[NB][2];
-                float2 vp[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) vp[h] = lds_half2(vs + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
+                for (int h = 0; h < 2; ++h) {
+                    const float2 vp = lds_half2(my_stage + G::CHUNK + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
+                    const float sc = vp.x * kPScale;
+                    float x[2];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float z = pr[b][i] * vp[i >> 1].y;
-                        x[i] = pr[b][i] * (vp[i >> 1].x * kPScale);
-                        if (!whole && !sees(b, i)) x[i] = z = 0.f;
-                        zacc[b][w][i & 1] += z;
-                        x[i] -= __uint_as_float(__float_as_uint(x[i]) & lo_mask);
+                    for (int e = 0; e < 2; ++e) {
+                        const float pe = pr[2 * h + e];
+                        x[e] = pe * sc;
+                        if constexpr (MASKED) {  // the parameters of a hidden key may be anything
+                            if (sees(2 * h + e)) zacc[w][e] = fmaf(pe, vp.y, zacc[w][e]);
+                            else x[e] = 0.f;
+                        } else {
+                            zacc[w][e] = fmaf(pe, vp.y, zacc[w][e]);
+                        }
                     }
-                    // bf16 by cutting off: exact for the high half, 2^-16 of x for the low one
-                    pb[b][0] = movmatrix_t(prmt(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x7632));
-                    pb[b][1] = movmatrix_t(prmt(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x7632));
+                    // bf16 halves: the first cuts x off (the rest is exact in fp32), the second cuts the
+                    // rest off: 16 bits together
+                    const uint32_t hi = prmt(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x7632);
+                    const float r0 = x[0] - __uint_as_float(hi << 16), r1 = x[1] - __uint_as_float(hi & 0xffff0000u);
+                    ph[w][h] = movmatrix_t(hi);
+                    pl[w][h] = movmatrix_t(prmt(__float_as_uint(r0), __float_as_uint(r1), 0x7632));
+                    if constexpr (KB > 1) pl[w][h] = __shfl_xor_sync(0xffffffffu, pl[w][h], 16);  // to column g ^ 4
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                if (MASKED && k > 0 && k >= n_here) break;
+                const uint32_t vs = stage + k * G::BYTES + G::CHUNK;
+                uint32_t v[4][NW];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 2 * t + (i & 1) + 8 * (i >> 1), at = r * (D / 2) + g * 4 * NW;
+                    lds_words(v[i], vs + (D == 128 ? at ^ (t << 5) : at));
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {  // nibbles 0-3, 4-7 of two tokens side by side
-                    const uint32_t x = prmt(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
-                    const uint32_t y = prmt(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
-                    const uint32_t a1[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
-                    const uint32_t a2[4] = {(x >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u, (y >> 8) & 0x000f000fu,
-                                            (y >> 8) & 0x00f000f0u};
+                for (int w = 0; w < NW; ++w) {
+                    uint32_t b[2];
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        mma_16816_bf16(o[b][4 * w + 2 * h], a1, pb[b][0], pb[b][1]);
-                        mma_16816_bf16(o[b][4 * w + 2 * h + 1], a2, pb[b][0], pb[b][1]);
+                    for (int h = 0; h < 2; ++h) {
+                        b[h] = ph[w][h];
+                        if constexpr (KB > 1) b[h] = g / SL == k ? ph[w][h] : (g ^ 4) / SL == k ? pl[w][h] : 0u;
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {  // nibbles 0-3, 4-7 of two tokens side by side
+                        const uint32_t x = prmt(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
+                        const uint32_t y = prmt(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
+                        const uint32_t a1[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+                        const uint32_t a2[4] = {(x >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u, (y >> 8) & 0x000f000fu,
+                                                (y >> 8) & 0x00f000f0u};
+                        mma_16816_bf16(o[4 * w + 2 * h], a1, b[0], b[1]);
+                        mma_16816_bf16(o[4 * w + 2 * h + 1], a2, b[0], b[1]);
+                        if constexpr (KB == 1) {
+                            mma_16816_bf16(o[4 * w + 2 * h], a1, pl[w][0], pl[w][1]);
+                            mma_16816_bf16(o[4 * w + 2 * h + 1], a2, pl[w][0], pl[w][1]);
+                        }
                     }
                 }
             }
         } else {
-            uint32_t pb[NB][2];
+            uint32_t ph[2], pl[2];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t hi, lo;
-                    split_h2(pr[b][2 * h], pr[b][2 * h + 1], hi, lo);
-                    pb[b][h] = movmatrix_t(t < 2 ? hi : lo);
-                }
+            for (int h = 0; h < 2; ++h) {
+                split_h2(pr[2 * h], pr[2 * h + 1], ph[h], pl[h]);
+                ph[h] = movmatrix_t(ph[h]);
+                pl[h] = movmatrix_t(pl[h]);
+            }
             const int r = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 uint32_t a[4];
                 const int c = 2 * i + ((lane >> 3) & 1);
-                ldsm_x4_t(vs + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) mma_16816(o[b][i], a, pb[b][0], pb[b][1]);
+                ldsm_x4_t(stage + G::CHUNK + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
+                mma_16816(o[i], a, ph[0], ph[1]);
+                mma_16816(o[i], a, pl[0], pl[1]);
             }
         }
+    };
+
+    uint32_t stage = ring;
+    for (int n = 0; n < mine; n += KB) {
+        cp_async_wait<0>();
+        __syncwarp();  // every lane's copies of these blocks are there, and every lane is done with the last ones
+        const uint32_t next = stage == ring ? ring + STAGE : ring;
+        issue(n + KB, next);
+        const int i = i0 + n + kb;
+        const int j0 = (i < nb_sink ? i : i + past_sinks) * 16;
+        bool present = n + kb < mine;
+        const bool whole = present && j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks) && !bad_id;
+        if (__all_sync(0xffffffffu, whole)) {
+            blocks(std::false_type{}, stage, KB, j0, true);
+        } else {
+            if (bad_id && present) {
+                const int id = table_id(n + kb);
+                present = id >= 0 && id < p.num_blocks;
+            }
+            blocks(std::true_type{}, stage, min(KB, mine - n), j0, present);
+        }
+        stage = next;
     }
-    cp_async_wait<0>();
     __syncwarp();  // the ring becomes the warp's partial output
 
-    // fold: halves and lanes, then warps of the CTA, then CTAs of the cluster
-    float* part = reinterpret_cast<float*>(smem + warp * ST * G::BYTES);  // [SL][D]
+    // fold: lanes and column groups, then warps of the CTA, then CTAs of the cluster
+    float* part = reinterpret_cast<float*>(smem + warp * 2 * STAGE);  // [SL][D]
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int e = 0; e < 2; ++e) {
+        const int sl = (2 * t + e) % SL;
+        if (ctx[e] == 0) l[e] = 0.f;  // a row without keys in a tile of rows that have some
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int sl = 4 * b + 2 * (t & 1) + e;
-            if (ctx[b][e] == 0) l[b][e] = 0.f;  // a row without keys in a tile of rows that have some
+        for (int x = SL / 2; x < 32; x <<= 1) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], x);
-#pragma unroll
-                for (int w = 0; w < NW; ++w) zacc[b][w][e] += __shfl_xor_sync(0xffffffffu, zacc[b][w][e], x);
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                float lo = o[b][i][e], hi = o[b][i][2 + e];  // rows g and g + 8 of the tile
-                lo += __shfl_xor_sync(0xffffffffu, lo, 2);
-                hi += __shfl_xor_sync(0xffffffffu, hi, 2);
-                int d0 = 16 * i + g, d1 = d0 + 8;
-                if constexpr (FMT == kWinQ4) {
-                    lo = fmaf(lo, kPUnscale, zacc[b][i >> 2][e]);
-                    hi = fmaf(hi, kPUnscale * 0.0625f, zacc[b][i >> 2][e]);
-                    d0 = 64 * (i >> 2) + 8 * g + 2 * (i & 3), d1 = d0 + 1;
-                }
-                if (t < 2) part[sl * D + d0] = lo, part[sl * D + d1] = hi;
-            }
-            if (lane < 2) s_ml[warp][sl][0] = m[b][e], s_ml[warp][sl][1] = l[b][e];
+            for (int w = 0; w < NW; ++w) zacc[w][e] += __shfl_xor_sync(0xffffffffu, zacc[w][e], x);
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            float lo = o[i][e], hi = o[i][2 + e];  // rows g and g + 8 of the tile
+#pragma unroll
+            for (int x = SL / 2; x < 4; x <<= 1) {
+                lo += __shfl_xor_sync(0xffffffffu, lo, x);
+                hi += __shfl_xor_sync(0xffffffffu, hi, x);
+            }
+            int d0 = 16 * i + g, d1 = d0 + 8;
+            if constexpr (FMT == kWinQ4) {
+                lo = fmaf(lo, kPUnscale, zacc[i >> 2][e]);
+                hi = fmaf(hi, kPUnscale * 0.0625f, zacc[i >> 2][e]);
+                d0 = 64 * (i >> 2) + 8 * g + 2 * (i & 3), d1 = d0 + 1;
+            }
+            if (kb == 0) part[sl * D + d0] = lo, part[sl * D + d1] = hi;
+        }
+        if (g == 0 && kb == 0) s_ml[warp][sl][0] = m[e], s_ml[warp][sl][1] = l[e];
+    }
     __syncthreads();
     const float* parts = reinterpret_cast<const float*>(smem);
-    constexpr int kPartStride = ST * G::BYTES / 4;
+    constexpr int kPartStride = 2 * STAGE / 4;
+    auto store = [&](int e, float v) {
+        const int r = e / D, d = e % D;
+        const size_t idx = ((size_t)(row0 + r / heads) * p.num_heads + kvh * p.group + h0 + r % heads) * D + d;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+        p.out[idx] = hi;
+        if (p.out_lo) p.out_lo[idx] = __float2bfloat16_rn(v - __bfloat162float(hi));
+    };
     for (int e = threadIdx.x; e < slots * D; e += W * 32) {
         const int r = e / D, d = e % D;
         float mx = s_ml[0][r][0];
@@ -595,11 +627,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
             }
         }
         if (splits == 1) {
-            const float v = sum == 0.f ? 0.f : acc / sum;
-            const size_t idx = ((size_t)(row0 + r / heads) * p.num_heads + kvh * p.group + h0 + r % heads) * D + d;
-            const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-            p.out[idx] = hi;
-            if (p.out_lo) p.out_lo[idx] = __float2bfloat16_rn(v - __bfloat162float(hi));
+            store(e, sum == 0.f ? 0.f : acc / sum);
         } else {
             reinterpret_cast<float*>(smem)[e] = acc;  // only this thread reads or writes the element
             if (d == 0) s_part[r][0] = mx, s_part[r][1] = sum;
@@ -608,7 +636,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
     if (splits == 1) return;
     cluster_sync();
     for (int e = (int)rank * W * 32 + threadIdx.x; e < slots * D; e += (int)splits * W * 32) {
-        const int r = e / D, d = e % D;
+        const int r = e / D;
         const uint32_t a_o = smem_u32(parts + e), a_m = smem_u32(&s_part[r][0]), a_l = smem_u32(&s_part[r][1]);
         float mx = -INFINITY;
         for (uint32_t c = 0; c < splits; ++c) mx = fmaxf(mx, ld_dsmem_f32(map_to_rank(a_m, c)));
@@ -623,23 +651,23 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
                 sum = lc;
             }
         }
-        const float v = sum == 0.f ? 0.f : acc / sum;
-        const size_t idx = ((size_t)(row0 + r / heads) * p.num_heads + kvh * p.group + h0 + r % heads) * D + d;
-        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-        p.out[idx] = hi;
-        if (p.out_lo) p.out_lo[idx] = __float2bfloat16_rn(v - __bfloat162float(hi));
+        store(e, sum == 0.f ? 0.f : acc / sum);
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int FMT, int D, int NB>
+template <int FMT, int D, int SL>
 inline int launch_window_rows(WinParams p, cudaStream_t st) {
-    constexpr int W = 4, ST = FMT == kWinQ4 ? 4 : 2, SL = 4 * NB;
-    constexpr int smem = W * ST * WinStage<FMT, D>::BYTES;
+    constexpr int W = 4;
+    constexpr int smem = W * 2 * (8 / SL) * WinStage<FMT, D>::BYTES;
     p.head_tiles = ceil_div(p.group, SL);
     p.qt = p.group >= SL ? 1 : SL / p.group;
     if (p.qt > p.S) p.qt = p.S;
     p.tiles = ceil_div(p.S, p.qt);
+    const long long block_bytes = (long long)p.num_layers * p.kv_heads * WinStage<FMT, D>::BYTES;
+    QTTS_REQUIRE(block_bytes < (1ll << 31), "paged attention: %lld bytes per block", block_bytes);
+    p.block_bytes = (uint32_t)block_bytes;
+    p.v_offset = (uint32_t)(p.kv_heads * WinStage<FMT, D>::CHUNK);
     const long long tiles = (long long)(p.R / p.S) * p.tiles * p.kv_heads * p.head_tiles;
     // keys one tile walks, at most
     const int limit = p.max_ctx < p.mbps * 16 ? p.max_ctx : p.mbps * 16;
@@ -649,7 +677,7 @@ inline int launch_window_rows(WinParams p, cudaStream_t st) {
     int splits = 1;
     while (splits < 16 && tiles * splits * 2 <= 4 * num_sms() && blocks >= 2 * W * splits * 2) splits *= 2;
     QTTS_REQUIRE(tiles * splits < (1ll << 31), "paged attention: %lld tiles", tiles);
-    constexpr auto kernel = paged_attn_window_kernel<FMT, D, NB, W, ST>;
+    constexpr auto kernel = paged_attn_window_kernel<FMT, D, SL, W>;
     QTTS_CHECK_CUDA((func_attr_once<kernel>(smem, true)));
     QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(tiles * splits)), dim3(W * 32), smem, st, dim3(splits, 1, 1), p));
     return QTTS_OK;
@@ -657,9 +685,14 @@ inline int launch_window_rows(WinParams p, cudaStream_t st) {
 
 template <int FMT, int D>
 inline int launch_window_attention(const WinParams& p, cudaStream_t st) {
-    // eight slots a tile where they can be filled: a block is then read once for twice the rows
-    if (p.group > 4 || (p.S > 1 && p.S * p.group > 4)) return launch_window_rows<FMT, D, 2>(p, st);
-    return launch_window_rows<FMT, D, 1>(p, st);
+    // the fp16 pool's blocks are four times the bytes for the same work, so that eight columns for
+    // one block cost it nothing; 4 bits: as few slots as the rows need, more blocks at once
+    if constexpr (FMT == kWinQ4) {
+        const int slots = p.S > 1 ? 8 : p.group;
+        if (slots <= 2) return launch_window_rows<FMT, D, 2>(p, st);
+        if (slots <= 4) return launch_window_rows<FMT, D, 4>(p, st);
+    }
+    return launch_window_rows<FMT, D, 8>(p, st);
 }
 
 }  // namespace qtts
