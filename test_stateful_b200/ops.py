@@ -118,59 +118,62 @@ def paged_attention_prefill(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, 
 
 
 # --------------------------------------------------------------------------- 4-bit KV cache, windowed attention
+# These wrappers sit on a decode step's launch path: each check is one cheap attribute read.
 _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
+_Strides = C.c_int64 * 3
 
 
-def _same_device(*ts) -> torch.device:
-    _need_cuda(*ts)
-    dev = ts[0].device
+def _same_device(*ts) -> int:
+    """Index of the CUDA device that holds every tensor (None skipped)."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
+    if dev < 0:
+        raise ValueError("libqtts_b200 kernels take CUDA tensors only")
     return dev
 
 
-class _on:
-    """Makes ``dev`` current while a kernel is launched (a no-op when it already is)."""
-
-    def __init__(self, dev: torch.device):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(dev: int, what: str, fn, *args):
+    """Calls an entry point with ``dev`` current and its current stream."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _lib.raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _need_i32(name: str, t: torch.Tensor, ndim: int):
-    if t.dtype != torch.int32 or t.dim() != ndim or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != ndim or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous int32 tensor of {ndim} dimension(s)")
 
 
 def _q4_dims(cache: torch.Tensor):
     """(blocks, layers, kv heads, head_dim) of a 4-bit pool."""
-    if cache.dtype != torch.uint8 or cache.dim() != 5 or cache.shape[2] != 2 or not cache.is_contiguous():
+    if cache.dtype is not torch.uint8 or cache.dim() != 5 or not cache.is_contiguous():
         raise ValueError("q4 cache: a contiguous uint8 tensor [blocks, layers, 2, kv_heads, 9 * head_dim]")
-    nb, L, _, H, chunk = cache.shape
-    if chunk not in (9 * 64, 9 * 128):
-        raise ValueError(f"q4 cache: {chunk} bytes per chunk (head_dim 64 has 576, 128 has 1152)")
+    nb, L, two, H, chunk = cache.shape
+    if two != 2 or chunk not in (9 * 64, 9 * 128):
+        raise ValueError(f"q4 cache: [.., 2, kv_heads, 9 * head_dim] with head_dim 64 or 128, got {tuple(cache.shape)}")
     return nb, L, H, chunk // 9
 
 
 def _q4_rows(name: str, t: torch.Tensor, n: int, layers: Optional[int], H: int, D: int):
-    """``[n, layers, H, D]`` view of K or V rows and its (token, layer, head) strides."""
-    if t.dim() == 3:
-        t = t.unsqueeze(1)
-    if t.dim() != 4 or t.shape[0] != n or t.shape[2:] != (H, D) or (layers is not None and t.shape[1] != layers):
+    """Layers, type and (token, layer, head) strides of K or V rows ``[n, (layers,) H, D]``."""
+    shape, st = t.shape, t.stride()
+    if len(shape) == 3:
+        shape, st = (shape[0], 1, shape[1], shape[2]), (st[0], 0, st[1], st[2])
+    if len(shape) != 4 or shape[0] != n or shape[2] != H or shape[3] != D or (layers or shape[1]) != shape[1]:
         raise ValueError(f"{name}: rows [{n}, {'layers' if layers is None else layers}, {H}, {D}], got {tuple(t.shape)}")
-    if t.dtype not in _DT:
+    dt = _DT.get(t.dtype)
+    if dt is None:
         raise ValueError(f"{name}: float16, bfloat16 or float32, got {t.dtype}")
-    if t.stride(3) != 1:
+    if st[3] != 1:
         raise ValueError(f"{name}: channels must be contiguous")
-    return t, (C.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+    # a dimension of one has no stride that matters
+    return shape[1], dt, _Strides(st[0] if n > 1 else 0, st[1] if shape[1] > 1 else 0, st[2] if H > 1 else 0)
 
 
 def kv_write_q4(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
@@ -181,15 +184,13 @@ def kv_write_q4(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapp
     dev = _same_device(cache, k, v, slot_mapping)
     nb, L, H, D = _q4_dims(cache)
     _need_i32("slot_mapping", slot_mapping, 1)
-    n = slot_mapping.numel()
-    k, ks = _q4_rows("k", k, n, None, H, D)
-    v, vs = _q4_rows("v", v, n, k.shape[1], H, D)
-    if k.dtype != v.dtype:
+    n = slot_mapping.shape[0]
+    layers, dt, ks = _q4_rows("k", k, n, None, H, D)
+    _, vdt, vs = _q4_rows("v", v, n, layers, H, D)
+    if dt != vdt:
         raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
-    with _on(dev):
-        rc = _lib.load().qtts_kv_write_q4(cache.data_ptr(), nb, L, H, D, k.data_ptr(), v.data_ptr(), _DT[k.dtype], ks,
-                                          vs, layer, k.shape[1], slot_mapping.data_ptr(), n, _lib.stream_ptr())
-    _lib.check(rc, "kv_write_q4")
+    _launch(dev, "kv_write_q4", _lib.load().qtts_kv_write_q4, cache.data_ptr(), nb, L, H, D, k.data_ptr(), v.data_ptr(),
+            dt, ks, vs, layer, layers, slot_mapping.data_ptr(), n)
 
 
 def kv_read_q4(cache: torch.Tensor, slot_mapping: torch.Tensor, layer: int = 0, n_layers: int = 1,
@@ -200,23 +201,21 @@ def kv_read_q4(cache: torch.Tensor, slot_mapping: torch.Tensor, layer: int = 0, 
     dev = _same_device(cache, slot_mapping, k, v)
     nb, L, H, D = _q4_dims(cache)
     _need_i32("slot_mapping", slot_mapping, 1)
-    n = slot_mapping.numel()
+    n = slot_mapping.shape[0]
     if dtype not in _DT:
         raise ValueError(f"kv_read_q4: float16, bfloat16 or float32, got {dtype}")
     if n_layers < 1 or layer < 0 or layer + n_layers > L:
         raise ValueError(f"kv_read_q4: layers [{layer}, +{n_layers}) of {L}")
     if k is None:
-        k = torch.empty(n, n_layers, H, D, device=dev, dtype=dtype)
+        k = torch.empty((n, n_layers, H, D), device=cache.device, dtype=dtype)
     if v is None:
-        v = torch.empty(n, n_layers, H, D, device=dev, dtype=k.dtype)
-    kr, ks = _q4_rows("k", k, n, n_layers, H, D)
-    vr, vs = _q4_rows("v", v, n, n_layers, H, D)
-    if kr.dtype != vr.dtype:
-        raise ValueError(f"k is {kr.dtype}, v is {vr.dtype}")
-    with _on(dev):
-        rc = _lib.load().qtts_kv_read_q4(cache.data_ptr(), nb, L, H, D, kr.data_ptr(), vr.data_ptr(), _DT[kr.dtype],
-                                         ks, vs, layer, n_layers, slot_mapping.data_ptr(), n, _lib.stream_ptr())
-    _lib.check(rc, "kv_read_q4")
+        v = torch.empty((n, n_layers, H, D), device=cache.device, dtype=k.dtype)
+    _, dt, ks = _q4_rows("k", k, n, n_layers, H, D)
+    _, vdt, vs = _q4_rows("v", v, n, n_layers, H, D)
+    if dt != vdt:
+        raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
+    _launch(dev, "kv_read_q4", _lib.load().qtts_kv_read_q4, cache.data_ptr(), nb, L, H, D, k.data_ptr(), v.data_ptr(), dt,
+            ks, vs, layer, n_layers, slot_mapping.data_ptr(), n)
     return k, v
 
 
@@ -227,43 +226,42 @@ def kv_gather_q4(cache: torch.Tensor, blocks: torch.Tensor, n_tokens: int,
     dev = _same_device(cache, blocks, out)
     nb, L, H, D = _q4_dims(cache)
     _need_i32("blocks", blocks, 1)
-    if n_tokens < 0 or n_tokens > 16 * blocks.numel():
-        raise ValueError(f"kv_gather_q4: {n_tokens} tokens of {blocks.numel()} blocks")
+    if n_tokens < 0 or n_tokens > 16 * blocks.shape[0]:
+        raise ValueError(f"kv_gather_q4: {n_tokens} tokens of {blocks.shape[0]} blocks")
     if out is None:
-        out = torch.empty(2 * L, H, n_tokens, D, device=dev, dtype=torch.float16)
-    elif out.dtype != torch.float16 or out.shape != (2 * L, H, n_tokens, D) or not out.is_contiguous():
+        out = torch.empty((2 * L, H, n_tokens, D), device=cache.device, dtype=torch.float16)
+    elif out.dtype is not torch.float16 or out.shape != (2 * L, H, n_tokens, D) or not out.is_contiguous():
         raise ValueError(f"kv_gather_q4: out must be contiguous fp16 [{2 * L}, {H}, {n_tokens}, {D}]")
-    with _on(dev):
-        rc = _lib.load().qtts_kv_gather_q4(cache.data_ptr(), nb, L, H, D, blocks.data_ptr(), n_tokens, out.data_ptr(),
-                                           _lib.stream_ptr())
-    _lib.check(rc, "kv_gather_q4")
+    _launch(dev, "kv_gather_q4", _lib.load().qtts_kv_gather_q4, cache.data_ptr(), nb, L, H, D, blocks.data_ptr(), n_tokens,
+            out.data_ptr())
     return out
 
 
-def _window_attention(what: str, q, kv, dims, layer, block_table, row_slot, row_ctx, max_ctx, window, sinks,
+def _window_attention(what, fn, q, kv, dims, layer, block_table, row_slot, row_ctx, max_ctx, window, sinks,
                       rows_per_stream, out, out_lo):
     dev = _same_device(q, kv, block_table, row_slot, row_ctx, out, out_lo)
     nb, L, H, D = dims
-    if q.dim() != 3 or q.dtype != torch.float32 or not q.is_contiguous() or q.shape[2] != D:
+    if q.dtype is not torch.float32 or q.dim() != 3 or not q.is_contiguous():
         raise ValueError(f"{what}: q must be contiguous float32 [rows, heads, {D}]")
-    R, Hq, _ = q.shape
+    R, Hq, qd = q.shape
+    if qd != D:
+        raise ValueError(f"{what}: head_dim {qd} over a pool of {D}")
     _need_i32("block_table", block_table, 2)
     _need_i32("row_slot", row_slot, 1)
     _need_i32("row_ctx", row_ctx, 1)
-    if row_slot.numel() != R or row_ctx.numel() != R:
-        raise ValueError(f"{what}: {R} query rows, {row_slot.numel()} slots and {row_ctx.numel()} contexts")
+    slots, mbps = block_table.shape
+    if row_slot.shape[0] != R or row_ctx.shape[0] != R:
+        raise ValueError(f"{what}: {R} query rows, {row_slot.shape[0]} slots and {row_ctx.shape[0]} contexts")
     if out is None:
-        out = torch.empty(R, Hq * D, device=dev, dtype=torch.bfloat16)
-    for o in (out, out_lo):
-        if o is not None and (o.dtype != torch.bfloat16 or o.numel() != R * Hq * D or not o.is_contiguous()):
-            raise ValueError(f"{what}: out and out_lo must be contiguous bfloat16 [{R}, {Hq * D}]")
-    with _on(dev):
-        rc = getattr(_lib.load(), "qtts_" + what)(q.data_ptr(), R, rows_per_stream, Hq, H, D, kv.data_ptr(), layer, L,
-                                                  16, nb, block_table.data_ptr(), block_table.shape[0],
-                                                  block_table.shape[1], row_slot.data_ptr(), row_ctx.data_ptr(),
-                                                  max_ctx, window, sinks, out.data_ptr(), _lib.ptr(out_lo),
-                                                  _lib.stream_ptr())
-    _lib.check(rc, what)
+        out = torch.empty((R, Hq * D), device=q.device, dtype=torch.bfloat16)
+    elif out.dtype is not torch.bfloat16 or out.numel() != R * Hq * D or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous bfloat16 [{R}, {Hq * D}]")
+    if out_lo is not None and (out_lo.dtype is not torch.bfloat16 or out_lo.numel() != R * Hq * D
+                               or not out_lo.is_contiguous()):
+        raise ValueError(f"{what}: out_lo must be contiguous bfloat16 [{R}, {Hq * D}]")
+    _launch(dev, what, fn, q.data_ptr(), R, rows_per_stream, Hq, H, D, kv.data_ptr(), layer, L, 16, nb,
+            block_table.data_ptr(), slots, mbps, row_slot.data_ptr(), row_ctx.data_ptr(), max_ctx, window, sinks,
+            out.data_ptr(), None if out_lo is None else out_lo.data_ptr())
     return out
 
 
@@ -277,12 +275,13 @@ def paged_attention_window(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, b
     zeros.  ``rows_per_stream`` > 1: the rows are streams of that many consecutive query tokens (a
     prompt chunk), which share the blocks they read.  Returns bf16 ``[R, Hq * D]`` (``out_lo``: its bf16
     residual)."""
-    if kv_pool.dtype != torch.float16 or kv_pool.dim() != 6 or kv_pool.shape[2] != 2 or kv_pool.shape[4] != 16 \
-            or not kv_pool.is_contiguous():
+    if kv_pool.dtype is not torch.float16 or kv_pool.dim() != 6 or not kv_pool.is_contiguous():
         raise ValueError("paged_attention_window: a contiguous float16 pool [blocks, layers, 2, kv_heads, 16, head_dim]")
-    nb, L, _, H, _, D = kv_pool.shape
-    return _window_attention("paged_attention_window", q, kv_pool, (nb, L, H, D), layer, block_table, row_slot, row_ctx,
-                             max_ctx, window, sinks, rows_per_stream, out, out_lo)
+    nb, L, two, H, bs, D = kv_pool.shape
+    if two != 2 or bs != 16:
+        raise ValueError(f"paged_attention_window: pool [.., 2, kv_heads, 16, head_dim], got {tuple(kv_pool.shape)}")
+    return _window_attention("paged_attention_window", _lib.load().qtts_paged_attention_window, q, kv_pool, (nb, L, H, D),
+                             layer, block_table, row_slot, row_ctx, max_ctx, window, sinks, rows_per_stream, out, out_lo)
 
 
 def paged_attention_q4(q: torch.Tensor, cache: torch.Tensor, layer: int, block_table: torch.Tensor,
@@ -291,8 +290,8 @@ def paged_attention_q4(q: torch.Tensor, cache: torch.Tensor, layer: int, block_t
                        out_lo: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`paged_attention_window` over a 4-bit pool ``cache [blocks, L, 2, Hkv, 9 D]`` (uint8, written by
     :func:`kv_write_q4`); every key is visible by default."""
-    return _window_attention("paged_attention_q4", q, cache, _q4_dims(cache), layer, block_table, row_slot, row_ctx,
-                             max_ctx, window, sinks, rows_per_stream, out, out_lo)
+    return _window_attention("paged_attention_q4", _lib.load().qtts_paged_attention_q4, q, cache, _q4_dims(cache), layer,
+                             block_table, row_slot, row_ctx, max_ctx, window, sinks, rows_per_stream, out, out_lo)
 
 
 def sample(logits: torch.Tensor, topk: int, gumbel: Optional[torch.Tensor] = None, temperature=None, penalty=None,
