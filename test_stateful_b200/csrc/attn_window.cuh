@@ -5,27 +5,29 @@
 // and gets softmax(q k^T / sqrt(D)) v over those keys; a row that sees none gets zeros.
 //
 // Row kernel.  One warp walks 16-token blocks, copied ahead of use into a ring of its own in shared
-// memory (cp.async, 16 bytes a lane).  The tensor work is mma.sync m16n8k16 with the keys on the M
-// side and (query, head) slots on the N side:
-//     S^T[16 tokens][8]   += K[16][16 channels] . Q^T       2 x D/16 instructions a block
-//     O^T[16 channels][8] += V^T[16][16 tokens] . P^T       D/16 or 2 x D/16 instructions a block
-// Both operands on the N side are pairs of 16-bit halves (what rounding took from the first is the
-// second), so that q and the probabilities keep 16 bits or more.  movmatrix turns the
-// probabilities from S^T's accumulator layout into the operand layout.
-// Decode tiles fill few of the eight columns (two query heads a KV head: two).  There the columns
-// are shared by KB = 8 / SL blocks of SL slots: q stands in every group of columns, so that each
-// lane of a quad finds the scores of one block in its registers and the softmax of KB blocks runs
-// at once, a block to a lane; for P V each block takes its own group's columns of P and the opposite
-// group's hold the second halves, the rest zero.  The column groups of O add up at the end.  (64
-// streams x 4096 keys, 4 bits: 388 instructions a block with one block at a time.)
+// memory (cp.async, 16 bytes a lane; K and V are separate steps of the ring).  The tensor work is
+// mma.sync with the keys on the M side and (query, head) slots on the N side:
+//     S^T[16 tokens][8]   += K[16][channels] . Q^T
+//     O^T[16 channels][8] += V^T[16][16 tokens] . P^T
+// q and the probabilities enter as pairs of a high part and what it leaves, so that they keep 16
+// bits or more; movmatrix turns the probabilities from S^T's accumulator layout into the operand
+// layout.
+// Decode tiles fill few of the eight columns (two query heads a KV head: two).  Over the 4-bit pool
+// the columns are shared by KB = 8 / SL blocks of SL slots: q stands in every group of columns, so that
+// each lane of a quad finds the scores of one block in its registers and the softmax of KB blocks
+// runs at once, a block to a lane; for P V each block takes its own group's columns of P, the opposite
+// group's hold the low parts, the rest zero.  The column groups of O add up at the end.
 //
-// 4-bit pool: a nibble masked out of a code word IS a small fp16 or bf16 number (a subnormal:
-// nibble << 0 = code * 2^-24 or 2^-133, nibble << 4 = 16 times that), so that no conversion is
-// needed; the powers of two move into q and the output, a token's scale into the score (K) and the
-// probability (V), and its zero multiplies sum(q) and p on the fp32 side.  The channel order of the
-// contractions is the one in which a lane's words arrive: lane (g, t) takes of K tokens g and g + 8
-// the channels 64 w + 16 t .. + 15, of V tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 the channels
-// 64 w + 8 g .. + 7.
+// 4-bit pool, K: the nibbles of a word are two words of bytes, (x << 4) & 0xf0f0f0f0 and x &
+// 0xf0f0f0f0, both 16 code: unsigned operands of an integer product (m16n8k32).  q is a 16-bit
+// fixed-point number in two signed digits, its unit 2^-16 of the slot's largest channel (far below the
+// error of a 4-bit key); the sum is exact.  A key's scale multiplies the sum, its zero sum(q).
+// V: a nibble masked out of a code word IS a small bf16 number (a subnormal: nibble << 0 = code *
+// 2^-133, nibble << 4 = 16 times that), so that no conversion is needed; the powers of two move
+// into p and the output, a token's scale into its probability, and its zero is added on the fp32 side.
+// The channel order of the contractions is the one in which a lane's words arrive: lane (g, t) takes
+// of K tokens g and g + 8 the channels 64 w + 16 t .. + 15, of V tokens 2 t, 2 t + 1, 2 t + 8,
+// 2 t + 9 the channels 64 w + 8 g .. + 7.
 #pragma once
 
 #include <type_traits>
@@ -56,19 +58,31 @@ struct WinParams {
 
 enum { kWinF16 = 0, kWinQ4 = 1 };
 
-__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+// D += A B, and D = A B for the first of a chain.  Not volatile: the compiler may interleave chains.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-
-// D = A B, the first of a chain
-__device__ __forceinline__ void mma_16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+}
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma_u8s8_first(int (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(0));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
 // transpose of an 8 x 8 matrix of 16-bit elements held as two per lane
@@ -103,39 +117,31 @@ __device__ __forceinline__ float2 lds_half2(uint32_t addr) {
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
-// A block's stage in shared memory: the K chunk, then the V chunk, 16-byte pieces permuted so that
-// the fragment reads meet no bank twice.
+// A chunk in shared memory, 16-byte pieces permuted so that the fragment reads meet no bank twice.
 //   fp16: rows of 2 D bytes read by ldmatrix; piece c of row r sits at c ^ (r % 8).
 //   4 bits: rows of D / 2 bytes; of D = 128 the eight pieces of two rows sit at L ^ 2 (r / 2 % 4):
 //   K reads two whole rows a quarter-warp, V one 16-channel stretch of rows 0, 2, 4, 6 (+ 1, + 8).
 template <int FMT, int D>
-struct WinStage {
+struct WinChunk {
     static constexpr int NW = D / 64;
-    static constexpr int CHUNK = FMT == kWinQ4 ? Q4Layout<D>::CHUNK : 32 * D;  // bytes of one (block, layer, k|v, head)
-    static constexpr int BYTES = 2 * CHUNK;
+    static constexpr int BYTES = FMT == kWinQ4 ? Q4Layout<D>::CHUNK : 32 * D;  // of one (block, layer, k|v, head)
 
-    // this lane's copies of one block
-    static __device__ __forceinline__ void copy(uint32_t dst, const uint8_t* k, const uint8_t* v, int lane) {
+    // this lane's copies
+    static __device__ __forceinline__ void copy(uint32_t dst, const uint8_t* src, int lane) {
         if constexpr (FMT == kWinQ4) {
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 const int j = lane + 32 * i, sw = D == 128 ? j ^ ((j >> 2) & 6) : j;
-                cp_async16(dst + sw * 16, k + j * 16);
-                cp_async16(dst + CHUNK + sw * 16, v + j * 16);
+                cp_async16(dst + sw * 16, src + j * 16);
             }
-            constexpr int PP = 4 * NW;  // pieces of (scale, zero) pairs
-            if (lane < 2 * PP) {
-                const int off = Q4Layout<D>::PARAMS + (lane & (PP - 1)) * 16;
-                cp_async16(dst + off + (lane < PP ? 0 : CHUNK), (lane < PP ? k : v) + off);
-            }
+            // the (scale, zero) pairs; their 4 NW pieces
+            if (lane < 4 * NW) cp_async16(dst + Q4Layout<D>::PARAMS + lane * 16, src + Q4Layout<D>::PARAMS + lane * 16);
         } else {
             constexpr int PR = D / 8;  // pieces per row
 #pragma unroll
             for (int i = 0; i < 16 * PR / 32; ++i) {
                 const int j = lane + 32 * i, r = j / PR, c = j % PR;
-                const int sw = r * PR + (c ^ (r & 7));
-                cp_async16(dst + sw * 16, k + j * 16);
-                cp_async16(dst + CHUNK + sw * 16, v + j * 16);
+                cp_async16(dst + (r * PR + (c ^ (r & 7))) * 16, src + j * 16);
             }
         }
     }
@@ -147,16 +153,16 @@ struct WinStage {
 constexpr float kPScale = 1.2676506002282294e30f;  // 2^100
 constexpr float kPUnscale = 8589934592.f;          // 2^133 / 2^100
 
-// SL slots a tile, W warps per CTA, two stages of KB blocks per warp.
-template <int FMT, int D, int SL, int W>
-__global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinParams p) {
-    using G = WinStage<FMT, D>;
+// SL slots a tile, W warps per CTA, NBUF steps of KB chunks in a warp's ring, at least MINB CTAs an SM.
+template <int FMT, int D, int SL, int W, int NBUF, int MINB>
+__global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const WinParams p) {
+    using G = WinChunk<FMT, D>;
     constexpr int NW = G::NW, MT = D / 16, KB = 8 / SL;
-    constexpr int STAGE = KB * G::BYTES;
+    constexpr int STEP = KB * G::BYTES, RING = NBUF * STEP;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_ml[W][SL][2];
     __shared__ float s_part[SL][2];  // the CTA's (max, sum) per slot
-    static_assert(SL * D * 4 <= 2 * STAGE, "a warp's partial output replaces its ring");
+    static_assert(SL * D * 4 <= RING, "a warp's partial output replaces its ring");
 
     griddep_wait();
     griddep_launch();
@@ -210,17 +216,18 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
 
     // ids of the warp's next 32 blocks, one per lane
     const int32_t* table = p.block_table + (size_t)(slot_ok ? slot : 0) * p.mbps;
-    const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::CHUNK;
-    const uint32_t ring = smem_u32(smem) + warp * 2 * STAGE;
+    const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::BYTES;
+    const uint32_t ring = smem_u32(smem) + warp * RING;
     int ids = 0;
     bool bad_id = false;  // an id outside the pool came up: its keys are hidden
     auto table_id = [&](int n) {  // of the warp's block n
         const int i = i0 + n;
         return __ldg(table + (i < nb_sink ? i : i + past_sinks));
     };
-    auto issue = [&](int n, uint32_t stage) {  // copy blocks n .. n + KB - 1; every lane commits a group, full or empty
+    // copy the K (v = 0) or V chunks of blocks n .. n + KB - 1; every lane commits a group, full or empty
+    auto issue = [&](int n, int v, uint32_t buf) {
         if (n < mine) {
-            if ((n & 31) == 0) {
+            if (v == 0 && (n & 31) == 0) {
                 ids = n + lane < mine ? table_id(n + lane) : 0;
                 const bool out = ids < 0 || ids >= p.num_blocks;
                 if (__any_sync(0xffffffffu, out)) bad_id = true;
@@ -229,31 +236,35 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
                     ids = 0;
                 }
             }
+            const uint8_t* from = base + (v ? p.v_offset : 0);
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
                 if (k > 0 && n + k >= mine) break;
-                const uint8_t* c = base + (uint64_t)(uint32_t)__shfl_sync(0xffffffffu, ids, (n & 31) + k) * p.block_bytes;
-                G::copy(stage + k * G::BYTES, c, c + p.v_offset, lane);
+                const uint32_t id = (uint32_t)__shfl_sync(0xffffffffu, ids, (n & 31) + k);
+                G::copy(buf + k * G::BYTES, from + (uint64_t)id * p.block_bytes, lane);
             }
         }
         cp_async_commit();
     };
-    issue(0, ring);
+    // steps are K, V, K, V, ...; step h lives in buffer h % NBUF, and NBUF - 1 are under way
+#pragma unroll
+    for (int h = 0; h < NBUF - 1; ++h) issue((h >> 1) * KB, h & 1, ring + h * STEP);
 
-    // Q^T operand.  Each slot's q is scaled by a power of two that brings its largest channel to
-    // [2^11, 2^12), so that fp16 halves hold it whatever its size; the upper nibbles' channels take
-    // 1/16.  Lane (g, t) holds column g: slot g % SL.
-    uint32_t qb[MT][2], ql[MT][2];
+    // Q^T operand: lane (g, t) holds column g, slot g % SL.
+    //   fp16: q scaled by a power of two that brings the slot's largest channel to [2^11, 2^12), so
+    //   that two fp16 halves hold it whatever its size.
+    //   4 bits: q / (largest channel) * 32639 rounded to an integer = 256 high + low, digits in [-128, 127].
+    constexpr int NQ = FMT == kWinQ4 ? 2 * NW : MT;
+    uint32_t qh[NQ][2], ql[NQ][2];
     float sf[2], qsum[NW][2];  // of this lane's score columns: accumulator -> log2 units, sum of q
     {
         const int s = g % SL;
         const bool valid = s < slots;
         const float* qr = p.q + ((size_t)(row0 + (valid ? s / heads : 0)) * p.num_heads + kvh * p.group + h0 +
                                  (valid ? s % heads : 0)) * D;
-        float v[NW][16], sum[NW], amax = 0.f;
+        float v[NW][16], amax = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            sum[w] = 0.f;
+        for (int w = 0; w < NW; ++w)
 #pragma unroll
             for (int c = 0; c < (FMT == kWinQ4 ? 4 : 8); ++c) {
                 if constexpr (FMT == kWinQ4) {
@@ -267,40 +278,56 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
                 }
             }
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-                amax = fmaxf(amax, fabsf(v[w][c]));
-                sum[w] += v[w][c];
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) amax = max_nan(amax, fabsf(v[w][c]));
+        amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float f;
+        if constexpr (FMT == kWinQ4) {
+            // a q that is zero everywhere (or below what a reciprocal holds) scores zero; one that is
+            // not finite makes its scores NaN through f
+            const float up = amax >= 1e-30f ? 32639.f / amax : 0.f;
+            f = amax * (1.f / (32639.f * 16.f)) * p.scale_log2;
+            if (!(amax < INFINITY)) f = __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                float sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) sum += v[w][c];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    qsum[w][e] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e)) * p.scale_log2;
+#pragma unroll
+                    for (int odd = 0; odd < 2; ++odd) {  // nibbles 0, 2, 4, 6 and 1, 3, 5, 7 of word e
+                        uint32_t hi = 0, lo = 0;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int x = __float2int_rn(v[w][8 * e + 2 * c + odd] * up), h = (x + 128) >> 8;
+                            hi |= (uint32_t)(h & 255) << (8 * c);
+                            lo |= (uint32_t)((x - 256 * h) & 255) << (8 * c);
+                        }
+                        qh[2 * w + odd][e] = hi;
+                        ql[2 * w + odd][e] = lo;
+                    }
+                }
             }
+        } else {
+            const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
+            const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
+            f = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = 4 * (i & 3) + 2 * h;
+                    split_h2(v[i >> 2][c] * up, v[i >> 2][c + 1] * up, qh[i][h], ql[i][h]);
+                }
         }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
-        const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
-        float f = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
-        if constexpr (FMT == kWinQ4) f *= 16777216.f;  // 2^24
 #pragma unroll
         for (int e = 0; e < 2; ++e) sf[e] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + e));
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 1);
-            sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 2);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) qsum[w][e] = __shfl_sync(0xffffffffu, sum[w], 4 * (2 * t + e)) * p.scale_log2;
-#pragma unroll
-            for (int s4 = 0; s4 < 4; ++s4) {
-                float x[4];
-                if constexpr (FMT == kWinQ4) {  // nibbles (2 h, 2 h + 4), (2 h + 1, 2 h + 5) of word s4 / 2, h = s4 % 2
-                    const int c = 8 * (s4 >> 1) + 2 * (s4 & 1);
-                    x[0] = v[w][c] * up, x[1] = v[w][c + 4] * up;
-                    x[2] = v[w][c + 1] * (up * 0.0625f), x[3] = v[w][c + 5] * (up * 0.0625f);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) x[c] = v[w][4 * s4 + c] * up;
-                }
-                split_h2(x[0], x[1], qb[4 * w + s4][0], ql[4 * w + s4][0]);
-                split_h2(x[2], x[3], qb[4 * w + s4][1], ql[4 * w + s4][1]);
-            }
-        }
     }
 
     float o[MT][4];  // FMT q4: row tile 4 w + k holds channels 64 w + 8 g + 2 k (c 0, 1) and + 1 (c 2, 3)
@@ -312,119 +339,110 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
 #pragma unroll
     for (int w = 0; w < NW; ++w) zacc[w][0] = zacc[w][1] = 0.f;
 
-    // one iteration's blocks (n_here of them) in a stage; MASKED: some row does not see all of them.
+    uint32_t buf = ring;      // of the step at hand
+    uint32_t ahead = ring + (NBUF - 1) * STEP;  // ... and of the one that is issued at it
+    auto turn = [&](int n, int v) {  // begin step (n, v): its chunks are there, the last step's buffer is free
+        cp_async_wait<NBUF - 2>();
+        __syncwarp();
+        issue(n + (NBUF - 1 + v) / 2 * KB, (NBUF - 1 + v) & 1, ahead);
+    };
+    auto next_step = [&]() {
+        ahead = buf;
+        buf = buf + STEP == ring + RING ? ring : buf + STEP;
+    };
+
+    // one iteration's blocks (n .. n + n_here - 1); MASKED: some row does not see all of them.
     // j0: first token of this lane's block; present: it is there and in the pool
-    auto blocks = [&](auto masked, const uint32_t stage, const int n_here, const int j0, const bool present) {
+    auto blocks = [&](auto masked, const int n, const int n_here, const int j0, const bool present) {
         constexpr bool MASKED = decltype(masked)::value;
         auto sees = [&](int i) {  // score i: token g + 8 (i / 2) of block kb, column 2 t + i % 2
             const int j = j0 + g + 8 * (i >> 1), c = ctx[i & 1];
             return present && j < c && (j >= c - window || j < p.sinks);
         };
-        const uint32_t my_stage = stage + kb * G::BYTES;
 
         // S^T, relative to mu
         float s[4];
         if constexpr (FMT == kWinQ4) {
-            float acc[NW][4];
+            int acc[NW][4];
+            constexpr int KI = KB > 1 ? 2 : 1;  // blocks whose chains of instructions run interleaved
 #pragma unroll
-            for (int k = 0; k < KB; ++k) {
-                if (MASKED && k > 0 && k >= n_here) break;
-                const uint32_t ks = stage + k * G::BYTES;
-                uint32_t kg[2 * NW], kh[2 * NW];  // tokens g, g + 8
+            for (int k0 = 0; k0 < KB; k0 += KI) {
+                if (MASKED && k0 > 0 && k0 >= n_here) break;
+                uint32_t kw[KI][2][2 * NW];  // tokens g and g + 8
                 const int row = g * (D / 2) + t * 8 * NW;
                 const int sw = D == 128 ? row ^ (((g >> 1) & 3) << 5) : row;
-                lds_words(kg, ks + sw);
-                lds_words(kh, ks + sw + 8 * (D / 2));
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    float d[4];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t x = kg[e * NW + w], y = kh[e * NW + w];
-                        const uint32_t a1[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
-                        const uint32_t a2[4] = {(x >> 8) & 0x000f000fu, (y >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u,
-                                                (y >> 8) & 0x00f000f0u};
-                        const int q1 = 4 * w + 2 * e, q2 = q1 + 1;
-                        if (e == 0) mma_16816_zero(d, a1, qb[q1][0], qb[q1][1]);
-                        else mma_16816(d, a1, qb[q1][0], qb[q1][1]);
-                        mma_16816(d, a2, qb[q2][0], qb[q2][1]);
-                        mma_16816(d, a1, ql[q1][0], ql[q1][1]);
-                        mma_16816(d, a2, ql[q2][0], ql[q2][1]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (k == 0 || kb == k) acc[w][i] = d[i];
+                for (int k = 0; k < KI; ++k) {
+                    lds_words(kw[k][0], buf + (k0 + k) * G::BYTES + sw);
+                    lds_words(kw[k][1], buf + (k0 + k) * G::BYTES + sw + 8 * (D / 2));
                 }
+                int d[KI][NW][4];
+                uint32_t a[2][KI][NW][4];  // even and odd nibbles, times 16
+#pragma unroll
+                for (int k = 0; k < KI; ++k)
+#pragma unroll
+                    for (int w = 0; w < NW; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t x = kw[k][i & 1][(i >> 1) * NW + w];
+                            a[0][k][w][i] = (x << 4) & 0xf0f0f0f0u;
+                            a[1][k][w][i] = x & 0xf0f0f0f0u;
+                        }
+#pragma unroll
+                for (int step = 0; step < 4; ++step)  // high digits of both nibbles, then low ones
+#pragma unroll
+                    for (int k = 0; k < KI; ++k)
+#pragma unroll
+                        for (int w = 0; w < NW; ++w) {
+                            if (step == 2)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) d[k][w][i] *= 256;
+                            if (step == 0) mma_u8s8_first(d[k][w], a[0][k][w], qh[2 * w]);
+                            else mma_u8s8(d[k][w], a[step & 1][k][w], step < 2 ? qh[2 * w + 1] : ql[2 * w + (step & 1)]);
+                        }
+#pragma unroll
+                for (int k = 0; k < KI; ++k)
+#pragma unroll
+                    for (int w = 0; w < NW; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (k0 + k == 0 || kb == k0 + k) acc[w][i] = d[k][w][i];
             }
             float2 kp[NW][2];
 #pragma unroll
             for (int w = 0; w < NW; ++w)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    kp[w][h] = lds_half2(my_stage + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
+                    kp[w][h] = lds_half2(buf + kb * G::BYTES + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float d = acc[0][i] * kp[0][i >> 1].x;
+                float d = (float)acc[0][i] * kp[0][i >> 1].x;
                 float z = fmaf(qsum[0][i & 1], kp[0][i >> 1].y, -mu[i & 1]);
                 if constexpr (NW == 2) {
-                    d = fmaf(acc[1][i], kp[1][i >> 1].x, d);
+                    d = fmaf((float)acc[1][i], kp[1][i >> 1].x, d);
                     z = fmaf(qsum[1][i & 1], kp[1][i >> 1].y, z);
                 }
                 s[i] = fmaf(d, sf[i & 1], z);
             }
         } else {
-            float acc[2][4];  // two chains
+            float acc[4][4];  // independent chains: even and odd steps, each half of q
             const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 uint32_t a[4];
                 const int c = 2 * i + (lane >> 4);
-                ldsm_x4(stage + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
-                if (i < 2) mma_16816_zero(acc[i & 1], a, qb[i][0], qb[i][1]);
-                else mma_16816(acc[i & 1], a, qb[i][0], qb[i][1]);
-                mma_16816(acc[i & 1], a, ql[i][0], ql[i][1]);
+                ldsm_x4(buf + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
+                if (i < 2) mma_f16_first(acc[i & 1], a, qh[i]), mma_f16_first(acc[2 + (i & 1)], a, ql[i]);
+                else mma_f16(acc[i & 1], a, qh[i]), mma_f16(acc[2 + (i & 1)], a, ql[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = fmaf(acc[0][i] + acc[1][i], sf[i & 1], -mu[i & 1]);
+            for (int i = 0; i < 4; ++i)
+                s[i] = fmaf((acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]), sf[i & 1], -mu[i & 1]);
         }
-
         if constexpr (MASKED) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (!sees(i)) s[i] = -INFINITY;
-            if constexpr (FMT == kWinF16) {
-                // a key that some row does not see must not reach it through 0 * V: what is not
-                // finite in such a row of V is set to zero, and the rows that do see it become NaN
-                const int r = lane >> 1, j = j0 + r;
-                const bool all = present && j < cmin && (j >= cmax - window || j < p.sinks);
-                bool bad = false;
-                if (!all) {
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        const uint32_t at = stage + G::CHUNK + (r * (D / 8) + (((lane & 1) * (D / 16) + c) ^ (r & 7))) * 16;
-                        uint32_t u[4];
-                        lds_words(u, at);
-                        bool here = false;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if ((u[x] & 0x7c00u) == 0x7c00u) u[x] &= 0xffff0000u, here = true;
-                            if ((u[x] & 0x7c000000u) == 0x7c000000u) u[x] &= 0x0000ffffu, here = true;
-                        }
-                        if (here)
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(u[0]), "r"(u[1]),
-                                         "r"(u[2]), "r"(u[3])
-                                         : "memory");
-                        bad |= here;
-                    }
-                }
-                const unsigned rows = __ballot_sync(0xffffffffu, bad);
-                if (rows) {
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (((rows >> (2 * (g + 8 * (i >> 1)))) & 3) && sees(i)) l[i & 1] = __int_as_float(0x7fffffff);
-                }
-            }
         }
 
         // softmax in the log2 domain; the running maximum moves only when a score passes it by
@@ -462,6 +480,42 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
             l[i & 1] += pr[i];
         }
 
+        next_step();
+        turn(n, 1);
+        if constexpr (MASKED && FMT == kWinF16) {
+            // a key that some row does not see must not reach it through 0 * V: what is not finite in
+            // such a row of V is set to zero, and the rows that do see it become NaN
+            const int r = lane >> 1, j = j0 + r;
+            const bool all = present && j < cmin && (j >= cmax - window || j < p.sinks);
+            bool bad = false;
+            if (!all) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const uint32_t at = buf + (r * (D / 8) + (((lane & 1) * (D / 16) + c) ^ (r & 7))) * 16;
+                    uint32_t u[4];
+                    lds_words(u, at);
+                    bool here = false;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        if ((u[x] & 0x7c00u) == 0x7c00u) u[x] &= 0xffff0000u, here = true;
+                        if ((u[x] & 0x7c000000u) == 0x7c000000u) u[x] &= 0x0000ffffu, here = true;
+                    }
+                    if (here)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+                                     "r"(u[3])
+                                     : "memory");
+                    bad |= here;
+                }
+            }
+            const unsigned rows = __ballot_sync(0xffffffffu, bad);
+            if (rows) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (((rows >> (2 * (g + 8 * (i >> 1)))) & 3) && sees(i)) l[i & 1] = __int_as_float(0x7fffffff);
+            }
+        }
+
         // O^T += V^T P^T
         if constexpr (FMT == kWinQ4) {
             uint32_t ph[NW][2], pl[NW][2];  // P^T operands of the KB blocks: column g belongs to block g / SL
@@ -469,7 +523,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
             for (int w = 0; w < NW; ++w) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float2 vp = lds_half2(my_stage + G::CHUNK + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
+                    const float2 vp = lds_half2(buf + kb * G::BYTES + Q4Layout<D>::PARAMS + w * 64 + (g + 8 * h) * 4);
                     const float sc = vp.x * kPScale;
                     float x[2];
 #pragma unroll
@@ -495,7 +549,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
                 if (MASKED && k > 0 && k >= n_here) break;
-                const uint32_t vs = stage + k * G::BYTES + G::CHUNK;
+                const uint32_t vs = buf + k * G::BYTES;
                 uint32_t v[4][NW];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -517,11 +571,11 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
                         const uint32_t a1[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
                         const uint32_t a2[4] = {(x >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u, (y >> 8) & 0x000f000fu,
                                                 (y >> 8) & 0x00f000f0u};
-                        mma_16816_bf16(o[4 * w + 2 * h], a1, b[0], b[1]);
-                        mma_16816_bf16(o[4 * w + 2 * h + 1], a2, b[0], b[1]);
+                        mma_bf16(o[4 * w + 2 * h], a1, b);
+                        mma_bf16(o[4 * w + 2 * h + 1], a2, b);
                         if constexpr (KB == 1) {
-                            mma_16816_bf16(o[4 * w + 2 * h], a1, pl[w][0], pl[w][1]);
-                            mma_16816_bf16(o[4 * w + 2 * h + 1], a2, pl[w][0], pl[w][1]);
+                            mma_bf16(o[4 * w + 2 * h], a1, pl[w]);
+                            mma_bf16(o[4 * w + 2 * h + 1], a2, pl[w]);
                         }
                     }
                 }
@@ -539,38 +593,35 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
             for (int i = 0; i < MT; ++i) {
                 uint32_t a[4];
                 const int c = 2 * i + ((lane >> 3) & 1);
-                ldsm_x4_t(stage + G::CHUNK + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
-                mma_16816(o[i], a, ph[0], ph[1]);
-                mma_16816(o[i], a, pl[0], pl[1]);
+                ldsm_x4_t(buf + (r * (D / 8) + (c ^ (r & 7))) * 16, a);
+                mma_f16(o[i], a, ph);
+                mma_f16(o[i], a, pl);
             }
         }
     };
 
-    uint32_t stage = ring;
     for (int n = 0; n < mine; n += KB) {
-        cp_async_wait<0>();
-        __syncwarp();  // every lane's copies of these blocks are there, and every lane is done with the last ones
-        const uint32_t next = stage == ring ? ring + STAGE : ring;
-        issue(n + KB, next);
+        turn(n, 0);
         const int i = i0 + n + kb;
         const int j0 = (i < nb_sink ? i : i + past_sinks) * 16;
         bool present = n + kb < mine;
         const bool whole = present && j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks) && !bad_id;
         if (__all_sync(0xffffffffu, whole)) {
-            blocks(std::false_type{}, stage, KB, j0, true);
+            blocks(std::false_type{}, n, KB, j0, true);
         } else {
             if (bad_id && present) {
                 const int id = table_id(n + kb);
                 present = id >= 0 && id < p.num_blocks;
             }
-            blocks(std::true_type{}, stage, min(KB, mine - n), j0, present);
+            blocks(std::true_type{}, n, min(KB, mine - n), j0, present);
         }
-        stage = next;
+        next_step();
     }
+    cp_async_wait<0>();
     __syncwarp();  // the ring becomes the warp's partial output
 
     // fold: lanes and column groups, then warps of the CTA, then CTAs of the cluster
-    float* part = reinterpret_cast<float*>(smem + warp * 2 * STAGE);  // [SL][D]
+    float* part = reinterpret_cast<float*>(smem + warp * RING);  // [SL][D]
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int sl = (2 * t + e) % SL;
@@ -601,7 +652,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
     }
     __syncthreads();
     const float* parts = reinterpret_cast<const float*>(smem);
-    constexpr int kPartStride = 2 * STAGE / 4;
+    constexpr int kPartStride = RING / 4;
     auto store = [&](int e, float v) {
         const int r = e / D, d = e % D;
         const size_t idx = ((size_t)(row0 + r / heads) * p.num_heads + kvh * p.group + h0 + r % heads) * D + d;
@@ -658,16 +709,18 @@ __global__ void __launch_bounds__(W * 32) paged_attn_window_kernel(const WinPara
 
 template <int FMT, int D, int SL>
 inline int launch_window_rows(WinParams p, cudaStream_t st) {
-    constexpr int W = 4;
-    constexpr int smem = W * 2 * (8 / SL) * WinStage<FMT, D>::BYTES;
+    constexpr int W = FMT == kWinQ4 ? 4 : 3, MINB = 4;
+    constexpr int NBUF = FMT == kWinQ4 ? (SL == 8 ? 6 : 3) : 4;
+    using G = WinChunk<FMT, D>;
+    constexpr int smem = W * NBUF * (8 / SL) * G::BYTES;
     p.head_tiles = ceil_div(p.group, SL);
     p.qt = p.group >= SL ? 1 : SL / p.group;
     if (p.qt > p.S) p.qt = p.S;
     p.tiles = ceil_div(p.S, p.qt);
-    const long long block_bytes = (long long)p.num_layers * p.kv_heads * WinStage<FMT, D>::BYTES;
+    const long long block_bytes = (long long)p.num_layers * 2 * p.kv_heads * G::BYTES;
     QTTS_REQUIRE(block_bytes < (1ll << 31), "paged attention: %lld bytes per block", block_bytes);
     p.block_bytes = (uint32_t)block_bytes;
-    p.v_offset = (uint32_t)(p.kv_heads * WinStage<FMT, D>::CHUNK);
+    p.v_offset = (uint32_t)(p.kv_heads * G::BYTES);
     const long long tiles = (long long)(p.R / p.S) * p.tiles * p.kv_heads * p.head_tiles;
     // keys one tile walks, at most
     const int limit = p.max_ctx < p.mbps * 16 ? p.max_ctx : p.mbps * 16;
@@ -677,7 +730,7 @@ inline int launch_window_rows(WinParams p, cudaStream_t st) {
     int splits = 1;
     while (splits < 16 && tiles * splits * 2 <= 4 * num_sms() && blocks >= 2 * W * splits * 2) splits *= 2;
     QTTS_REQUIRE(tiles * splits < (1ll << 31), "paged attention: %lld tiles", tiles);
-    constexpr auto kernel = paged_attn_window_kernel<FMT, D, SL, W>;
+    constexpr auto kernel = paged_attn_window_kernel<FMT, D, SL, W, NBUF, MINB>;
     QTTS_CHECK_CUDA((func_attr_once<kernel>(smem, true)));
     QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(tiles * splits)), dim3(W * 32), smem, st, dim3(splits, 1, 1), p));
     return QTTS_OK;
