@@ -162,6 +162,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_ml[W][SL][2];
     __shared__ float s_part[SL][2];  // the CTA's (max, sum) per slot
+    // Q^T operand words of (slot, t): high parts, then low parts; accumulator -> log2 units; sums of q
+    constexpr int NQ = FMT == kWinQ4 ? 2 * NW : MT;
+    __shared__ __align__(16) uint32_t s_q[SL][4][4 * NQ];
+    __shared__ float s_qf[SL], s_qsum[SL][NW];
     static_assert(SL * D * 4 <= RING, "a warp's partial output replaces its ring");
 
     griddep_wait();
@@ -182,6 +186,34 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     const int nq = min(p.qt, p.S - q0);
     const int row0 = stream * p.S + q0;
     const int slots = nq * heads;
+
+    // q of this warp's slots (warp, warp + W, ...), on its way while the contexts and block ids are read.
+    //   4 bits: lane = 16 w + 4 t + 2 e + odd takes the odd or even channels of word (w, t, e)
+    //   fp16: lane takes the channel pairs lane and lane + 32
+    constexpr int QS = (SL + W - 1) / W;
+    float qv[QS][4];
+#pragma unroll
+    for (int k = 0; k < QS; ++k) {
+        const int s = warp + k * W;
+        qv[k][0] = qv[k][1] = qv[k][2] = qv[k][3] = 0.f;
+        if (s < slots) {
+            const float* qr = p.q + ((size_t)(row0 + s / heads) * p.num_heads + kvh * p.group + h0 + s % heads) * D;
+            if constexpr (FMT == kWinQ4) {
+                if (lane < 16 * NW) {
+                    const float4 a = __ldg(reinterpret_cast<const float4*>(qr + 8 * (lane >> 1)));
+                    const float4 b = __ldg(reinterpret_cast<const float4*>(qr + 8 * (lane >> 1) + 4));
+                    qv[k][0] = lane & 1 ? a.y : a.x, qv[k][1] = lane & 1 ? a.w : a.z;
+                    qv[k][2] = lane & 1 ? b.y : b.x, qv[k][3] = lane & 1 ? b.w : b.z;
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float2 a = __ldg(reinterpret_cast<const float2*>(qr) + lane + 32 * w);
+                    qv[k][2 * w] = a.x, qv[k][2 * w + 1] = a.y;
+                }
+            }
+        }
+    }
 
     // contexts: this lane's score columns, and the tile's extremes over rows that see anything
     const int limit = min(p.max_ctx, p.mbps * 16);
@@ -250,39 +282,17 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
 #pragma unroll
     for (int h = 0; h < NBUF - 1; ++h) issue((h >> 1) * KB, h & 1, ring + h * STEP);
 
-    // Q^T operand: lane (g, t) holds column g, slot g % SL.
+    // Q^T operand, made once per CTA.
     //   fp16: q scaled by a power of two that brings the slot's largest channel to [2^11, 2^12), so
     //   that two fp16 halves hold it whatever its size.
     //   4 bits: q / (largest channel) * 32639 rounded to an integer = 256 high + low, digits in [-128, 127].
-    constexpr int NQ = FMT == kWinQ4 ? 2 * NW : MT;
-    uint32_t qh[NQ][2], ql[NQ][2];
-    float sf[2], qsum[NW][2];  // of this lane's score columns: accumulator -> log2 units, sum of q
-    {
-        const int s = g % SL;
-        const bool valid = s < slots;
-        const float* qr = p.q + ((size_t)(row0 + (valid ? s / heads : 0)) * p.num_heads + kvh * p.group + h0 +
-                                 (valid ? s % heads : 0)) * D;
-        float v[NW][16], amax = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w)
+    for (int k = 0; k < QS; ++k) {
+        const int s = warp + k * W;
+        if (s >= SL) break;
+        float amax = max_nan(max_nan(fabsf(qv[k][0]), fabsf(qv[k][1])), max_nan(fabsf(qv[k][2]), fabsf(qv[k][3])));
 #pragma unroll
-            for (int c = 0; c < (FMT == kWinQ4 ? 4 : 8); ++c) {
-                if constexpr (FMT == kWinQ4) {
-                    const float4 u = valid ? __ldg(reinterpret_cast<const float4*>(qr + 64 * w + 16 * t + 4 * c))
-                                           : make_float4(0.f, 0.f, 0.f, 0.f);
-                    v[w][4 * c] = u.x, v[w][4 * c + 1] = u.y, v[w][4 * c + 2] = u.z, v[w][4 * c + 3] = u.w;
-                } else {
-                    const float2 u = valid ? __ldg(reinterpret_cast<const float2*>(qr + 64 * w + 2 * t + 8 * c))
-                                           : make_float2(0.f, 0.f);
-                    v[w][2 * c] = u.x, v[w][2 * c + 1] = u.y;
-                }
-            }
-#pragma unroll
-        for (int w = 0; w < NW; ++w)
-#pragma unroll
-            for (int c = 0; c < 16; ++c) amax = max_nan(amax, fabsf(v[w][c]));
-        amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        for (int x = 1; x < 32; x <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, x));
         float f;
         if constexpr (FMT == kWinQ4) {
             // a q that is zero everywhere (or below what a reciprocal holds) scores zero; one that is
@@ -290,44 +300,53 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
             const float up = amax >= 1e-30f ? 32639.f / amax : 0.f;
             f = amax * (1.f / (32639.f * 16.f)) * p.scale_log2;
             if (!(amax < INFINITY)) f = __int_as_float(0x7fffffff);
+            float sum = (qv[k][0] + qv[k][1]) + (qv[k][2] + qv[k][3]);
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                float sum = 0.f;
+            for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            uint32_t hi = 0, lo = 0;
 #pragma unroll
-                for (int c = 0; c < 16; ++c) sum += v[w][c];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    qsum[w][e] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e)) * p.scale_log2;
-#pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) {  // nibbles 0, 2, 4, 6 and 1, 3, 5, 7 of word e
-                        uint32_t hi = 0, lo = 0;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int x = __float2int_rn(v[w][8 * e + 2 * c + odd] * up), h = (x + 128) >> 8;
-                            hi |= (uint32_t)(h & 255) << (8 * c);
-                            lo |= (uint32_t)((x - 256 * h) & 255) << (8 * c);
-                        }
-                        qh[2 * w + odd][e] = hi;
-                        ql[2 * w + odd][e] = lo;
-                    }
-                }
+            for (int c = 0; c < 4; ++c) {
+                const int x = __float2int_rn(qv[k][c] * up), h = (x + 128) >> 8;
+                hi |= (uint32_t)(h & 255) << (8 * c);
+                lo |= (uint32_t)((x - 256 * h) & 255) << (8 * c);
+            }
+            const int w = lane >> 4;
+            if (w < NW) {
+                uint32_t* dst = &s_q[s][(lane >> 2) & 3][2 * (2 * w + (lane & 1)) + ((lane >> 1) & 1)];
+                dst[0] = hi;
+                dst[2 * NQ] = lo;
+                if ((lane & 15) == 0) s_qsum[s][w] = sum * p.scale_log2;
             }
         } else {
             const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
             const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
             f = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int w = 0; w < NW; ++w) {
+                uint32_t hi, lo;
+                split_h2(qv[k][2 * w] * up, qv[k][2 * w + 1] * up, hi, lo);
+                const int pair = lane + 32 * w;  // channels 16 i + 8 h + 2 t: word 2 i + h of t
+                s_q[s][pair & 3][pair >> 2] = hi;
+                s_q[s][pair & 3][2 * NQ + (pair >> 2)] = lo;
+            }
+        }
+        if (lane == 0) s_qf[s] = f;
+    }
+    __syncthreads();
+    uint32_t qh[NQ][2], ql[NQ][2];     // of column g: slot g % SL
+    float sf[2], qsum[NW][2];          // of this lane's score columns
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c = 4 * (i & 3) + 2 * h;
-                    split_h2(v[i >> 2][c] * up, v[i >> 2][c + 1] * up, qh[i][h], ql[i][h]);
-                }
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            qh[i][h] = s_q[g % SL][t][2 * i + h];
+            ql[i][h] = s_q[g % SL][t][2 * NQ + 2 * i + h];
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) sf[e] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + e));
+    for (int e = 0; e < 2; ++e) {
+        sf[e] = s_qf[(2 * t + e) % SL];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) qsum[w][e] = FMT == kWinQ4 ? s_qsum[(2 * t + e) % SL][w] : 0.f;
     }
 
     float o[MT][4];  // FMT q4: row tile 4 w + k holds channels 64 w + 8 g + 2 k (c 0, 1) and + 1 (c 2, 3)

@@ -1,11 +1,14 @@
 """4-bit KV cache and windowed paged attention on the GPU against the float64 oracle.
 
 Tolerances.  The cache: codes and parameters bit for bit; values read back are one rounding (half a
-unit) of the stored value.  Attention, out + out_lo: q in two fp16 halves (2^-22), fp32 score sums,
-ex2.approx (2^-22), probabilities in two halves of 16 bits together (2^-16, the 4-bit pool) or 22
-(fp16 pool), the output in two bf16 halves (2^-17): a score is off by at most |q| |k| 2^-16 / sqrt(D) in
-sums of D <= 128 terms, below 2^-13 for the norms drawn here, so an output, a mean of values,
-is off by at most (2^-13 + 2^-15) max|v| < 2^-12 max|v|."""
+unit) of the stored value.  Attention, out + out_lo: fp32 score sums, ex2.approx (2^-22), probabilities
+in two halves of 16 bits together (2^-16, the 4-bit pool) or 22 (fp16 pool), the output in two bf16
+halves (2^-17): without q's own rounding a score is off by less than 2^-14 for the norms drawn here
+(D <= 128 fp32 terms), so an output, a mean of values, by at most (2^-13 + 2^-15) max|v| < 2^-12 max|v|.
+q is two fp16 halves (2^-22, covered by that) over the fp16 pool.  Over the 4-bit pool it is a 16-bit
+fixed-point number, each channel off by at most max|q| / 65278 (half a unit): a score by at most
+d = max|q| / 65278 sum|k| / sqrt(D), a probability by a factor within exp(+-2 d) (numerator and sum), an
+output by (exp(2 d) - 1) max|v| more."""
 
 
 import numpy as np
@@ -251,6 +254,14 @@ def _attend(fmt, *a, window=0, sinks=0, **kw):
     return ops.paged_attention_q4(*a, window=window, sinks=sinks, **kw)
 
 
+def _tolerance(fmt, q, kv):
+    """Absolute tolerance of out + out_lo for one row (see the module's docstring)."""
+    if not kv.size:
+        return 0.0
+    d = np.abs(q).max() / 65278 * np.abs(kv[0]).sum(-1).max() / np.sqrt(q.shape[-1]) if fmt == "q4" else 0.0
+    return (2.0 ** -12 + np.expm1(2 * d)) * np.abs(kv[1]).max()
+
+
 def _run_case(fmt, Hq, H, D, ctxs, S, window, sinks, seed=0, max_ctx=None, poison=None, qscale=1.0):
     """``ctxs``: each stream's last row's context.  Returns nothing; asserts against the oracle."""
     n = len(ctxs)
@@ -280,7 +291,7 @@ def _run_case(fmt, Hq, H, D, ctxs, S, window, sinks, seed=0, max_ctx=None, poiso
         for t in range(S):
             r = b * S + t
             want = O.attention(q[r].numpy(), kv[0], kv[1], min(int(row_ctx[r]), limit), window, sinks)
-            tol = 2.0 ** -12 * (np.abs(kv[1]).max() if kv.size else 0.0)
+            tol = _tolerance(fmt, q[r].numpy(), kv)
             assert np.abs(got[r] - want).max() <= tol, (r, np.abs(got[r] - want).max(), tol)
     return out
 
@@ -335,8 +346,8 @@ def test_row_ctx_is_capped_at_max_ctx(fmt):
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
 @pytest.mark.parametrize("qscale", [1e-6, 1e-3, 8.0])
 def test_query_magnitudes(fmt, qscale):
-    """Scores near 0 and up to some tens: |q| 8 times larger makes a score's error 8 times larger, and a
-    peaked row is a mean over few values; 2^-12 max|v| still covers 8 x 2^-16 x |q||k|/sqrt(D)."""
+    """Scores near 0 and up to some tens (fp32 sums of 8 times larger terms: below 2^-11 in the worst case of
+    all roundings aligned, 2^-15 at their spread, which 2^-12 max|v| covers for a mean over few values)."""
     _run_case(fmt, 4, 2, 64, [50, 130], 1, 0, 0, qscale=qscale)
 
 
@@ -396,7 +407,7 @@ def test_nan_key_inside_a_chunk_reaches_later_rows_only(fmt, S):
             want = O.attention(q[r].numpy(), kv[0], kv[1], int(ctxs[r]))
             # bf16 output alone: half a unit (2^-8 of the value), then the tolerance of the pair
             err = np.abs(out[r].double().numpy().reshape(-1) - want)
-            assert (err <= 2.0 ** -8 * np.abs(want) + 2.0 ** -12 * np.abs(kv[1]).max()).all()
+            assert (err <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[r].numpy(), kv)).all()
 
 
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
@@ -415,7 +426,7 @@ def test_bad_slots_and_blocks_are_reported(fmt):
     for r, blocks in ((0, [0, 1]), (3, [2]), (4, [3])):   # an id outside the pool hides its keys
         kv = vals[blocks, 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
         want = O.attention(q[r].numpy(), kv[0], kv[1], kv.shape[2])
-        assert (np.abs(out[r] - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -12 * np.abs(kv[1]).max()).all()
+        assert (np.abs(out[r] - want) <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[r].numpy(), kv)).all()
 
 
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
@@ -490,7 +501,7 @@ def test_pool_offsets_past_32_bits(fmt):
     out = _attend(fmt, q.to(DEV), pool, L - 1, blocks.view(1, 3).to(DEV), one, one + ctx, 48).double().cpu().numpy()
     kv = vals.transpose(1, 2, 0, 3, 4).reshape(2, H, 48, D)
     want = O.attention(q[0].numpy(), kv[0], kv[1], ctx)
-    assert (np.abs(out[0] - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -12 * np.abs(kv[1]).max()).all()
+    assert (np.abs(out[0] - want) <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[0].numpy(), kv)).all()
 
 
 # ------------------------------------------------------------------------------ as a server uses them
@@ -537,7 +548,7 @@ def test_streams_on_a_q4_pool():
             for s in (0, 1):
                 kv = np.concatenate(held[s])[:, 2 * layer:2 * layer + 2].transpose(1, 2, 0, 3)
                 want = O.attention(q[s].numpy(), kv[0], kv[1], kv.shape[2], window, sinks)
-                assert np.abs(out[s] - want).max() <= 2.0 ** -12 * np.abs(kv[1]).max()
+                assert np.abs(out[s] - want).max() <= _tolerance("q4", q[s].numpy(), kv)
     for s in (0, 1):
         n = sum(len(h) for h in held[s])
         _close_values(sch.gather(s, n), np.concatenate(held[s]).transpose(1, 2, 0, 3), torch.float16)
