@@ -153,6 +153,16 @@ struct WinChunk {
 constexpr float kPScale = 1.2676506002282294e30f;  // 2^100
 constexpr float kPUnscale = 8589934592.f;          // 2^133 / 2^100
 
+constexpr int kWinMaxSplits = 16;  // CTAs of a cluster
+
+// ld.shared::cluster that several of may be under way (no memory clobber): the data was published by
+// a cluster barrier
+__device__ __forceinline__ float ld_dsmem_now(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+
 // SL slots a tile, W warps per CTA, NBUF steps of KB chunks in a warp's ring, at least MINB CTAs an SM.
 template <int FMT, int D, int SL, int W, int NBUF, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const WinParams p) {
@@ -705,21 +715,28 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     }
     if (splits == 1) return;
     cluster_sync();
-    for (int e = (int)rank * W * 32 + threadIdx.x; e < slots * D; e += (int)splits * W * 32) {
-        const int r = e / D;
-        const uint32_t a_o = smem_u32(parts + e), a_m = smem_u32(&s_part[r][0]), a_l = smem_u32(&s_part[r][1]);
-        float mx = -INFINITY;
-        for (uint32_t c = 0; c < splits; ++c) mx = fmaxf(mx, ld_dsmem_f32(map_to_rank(a_m, c)));
-        float sum = 0.f, acc = 0.f;
-        for (uint32_t c = 0; c < splits; ++c) {
-            const float mc = ld_dsmem_f32(map_to_rank(a_m, c)), lc = ld_dsmem_f32(map_to_rank(a_l, c));
-            if (mc != -INFINITY) {
-                const float f = ex2_approx(mc - mx);
-                sum += lc * f;
-                acc += ld_dsmem_f32(map_to_rank(a_o, c)) * f;
-            } else if (lc != 0.f) {
-                sum = lc;
-            }
+    // a warp takes 32 channels of a slot; lane c fetches CTA c's (max, sum), every lane its channel of
+    // every CTA, all loads under way at once
+    for (int j = (int)rank * W + warp; j < slots * (D / 32); j += (int)splits * W) {
+        const int r = j / (D / 32), e = j * 32 + lane;
+        float mc = -INFINITY, lc = 0.f;
+        if (lane < (int)splits) {
+            mc = ld_dsmem_now(map_to_rank(smem_u32(&s_part[r][0]), lane));
+            lc = ld_dsmem_now(map_to_rank(smem_u32(&s_part[r][1]), lane));
+        }
+        float v[kWinMaxSplits];
+#pragma unroll
+        for (int c = 0; c < kWinMaxSplits; ++c)
+            if (c < (int)splits) v[c] = ld_dsmem_now(map_to_rank(smem_u32(parts + e), c));
+        const float mx = warp_max(mc);
+        const float f = mc == -INFINITY ? 0.f : ex2_approx(mc - mx);
+        // a CTA without keys holds nothing (0 f), one of nothing but NaN scores a sum that is not zero
+        const float sum = warp_sum(mc == -INFINITY && lc != 0.f ? lc : lc * f);
+        float acc = 0.f;
+#pragma unroll
+        for (int c = 0; c < kWinMaxSplits; ++c) {
+            const float fc = __shfl_sync(0xffffffffu, f, c);
+            if (c < (int)splits && fc != 0.f) acc = fmaf(v[c], fc, acc);
         }
         store(e, sum == 0.f ? 0.f : acc / sum);
     }
@@ -747,7 +764,7 @@ inline int launch_window_rows(WinParams p, cudaStream_t st) {
     if (p.window > 0 && (long long)p.window + p.sinks + p.qt + 32 < keys) keys = (long long)p.window + p.sinks + p.qt + 32;
     const int blocks = (int)((keys + 15) / 16);
     int splits = 1;
-    while (splits < 16 && tiles * splits * 2 <= 4 * num_sms() && blocks >= 2 * W * splits * 2) splits *= 2;
+    while (splits < kWinMaxSplits && tiles * splits * 2 <= 4 * num_sms() && blocks >= 2 * W * splits * 2) splits *= 2;
     QTTS_REQUIRE(tiles * splits < (1ll << 31), "paged attention: %lld tiles", tiles);
     constexpr auto kernel = paged_attn_window_kernel<FMT, D, SL, W, NBUF, MINB>;
     QTTS_CHECK_CUDA((func_attr_once<kernel>(smem, true)));
