@@ -743,12 +743,33 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
+template <int FMT, int D, int SL, int W, int MINB>
+inline int launch_window_rows_w(const WinParams& p, long long tiles, int splits, cudaStream_t st) {
+    // 4 bits: three steps of KB chunks (one iteration's K and V ahead of the step at hand); with one
+    // block a step, six, for the same bytes under way.  fp16: four steps of one 4 KB chunk.
+    constexpr int NBUF = FMT == kWinQ4 ? (SL == 8 ? 6 : 3) : 4;
+    constexpr int smem = W * NBUF * (8 / SL) * WinChunk<FMT, D>::BYTES;
+    constexpr auto kernel = paged_attn_window_kernel<FMT, D, SL, W, NBUF, MINB>;
+    QTTS_CHECK_CUDA((func_attr_once<kernel>(smem, true)));
+    QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(tiles * splits)), dim3(W * 32), smem, st, dim3(splits, 1, 1), p));
+    return QTTS_OK;
+}
+
+// How a tile's keys are shared.  16 warps fit an SM over the 4-bit pool, 12 over fp16; all variants
+// fill it, with fewer and larger CTAs the fewer tiles there are: warps of one CTA fold cheaper than
+// CTAs of a cluster.  Beyond the tiles that half-SM CTAs cover, a cluster splits a tile while every
+// warp keeps three blocks.  Measured (us, 16 heads over 8, rows x context, B200), warps x splits:
+//   4 bits  1 x 4000:  4 x 16 7.0   8 x 8 7.5    8 x 4 9.3    2 x 16 8.4
+//          16 x 520:   8 x 1 7.0    4 x 1 7.8    8 x 2 8.7    4 x 4 8.8
+//          64 x 520:   4 x 1 14.3   2 x 1 14.7   8 x 1 18.1   4 x 2 20.9
+//         128 x 520:   2 x 1 23.3   4 x 1 25.6   8 x 1 32.7
+//   fp16    1 x 4000:  6 x 8 9.9    3 x 16 9.7   6 x 4 13.5
+//          64 x 520:   3 x 1 27.3   6 x 1 29.1   2 x 1 29.7   3 x 2 33.3
+//         128 x 520:   3 x 1 48.1   2 x 1 57.3   6 x 1 53.5
 template <int FMT, int D, int SL>
 inline int launch_window_rows(WinParams p, cudaStream_t st) {
-    constexpr int W = FMT == kWinQ4 ? 4 : 3, MINB = 4;
-    constexpr int NBUF = FMT == kWinQ4 ? (SL == 8 ? 6 : 3) : 4;
     using G = WinChunk<FMT, D>;
-    constexpr int smem = W * NBUF * (8 / SL) * G::BYTES;
+    constexpr int WL = FMT == kWinQ4 ? 8 : 6;  // warps of a half-SM CTA
     p.head_tiles = ceil_div(p.group, SL);
     p.qt = p.group >= SL ? 1 : SL / p.group;
     if (p.qt > p.S) p.qt = p.S;
@@ -758,18 +779,22 @@ inline int launch_window_rows(WinParams p, cudaStream_t st) {
     p.block_bytes = (uint32_t)block_bytes;
     p.v_offset = (uint32_t)(p.kv_heads * G::BYTES);
     const long long tiles = (long long)(p.R / p.S) * p.tiles * p.kv_heads * p.head_tiles;
-    // keys one tile walks, at most
+    QTTS_REQUIRE(tiles * kWinMaxSplits < (1ll << 31), "paged attention: %lld tiles", tiles);
+    const int slots = 2 * num_sms();
+    if (tiles > slots) {
+        if constexpr (FMT == kWinQ4) {
+            if (tiles > 2 * slots) return launch_window_rows_w<FMT, D, SL, 2, 8>(p, tiles, 1, st);
+            return launch_window_rows_w<FMT, D, SL, 4, 4>(p, tiles, 1, st);
+        }
+        return launch_window_rows_w<FMT, D, SL, 3, 4>(p, tiles, 1, st);
+    }
+    // blocks one tile walks, at most
     const int limit = p.max_ctx < p.mbps * 16 ? p.max_ctx : p.mbps * 16;
     long long keys = limit;
     if (p.window > 0 && (long long)p.window + p.sinks + p.qt + 32 < keys) keys = (long long)p.window + p.sinks + p.qt + 32;
-    const int blocks = (int)((keys + 15) / 16);
     int splits = 1;
-    while (splits < kWinMaxSplits && tiles * splits * 2 <= 4 * num_sms() && blocks >= 2 * W * splits * 2) splits *= 2;
-    QTTS_REQUIRE(tiles * splits < (1ll << 31), "paged attention: %lld tiles", tiles);
-    constexpr auto kernel = paged_attn_window_kernel<FMT, D, SL, W, NBUF, MINB>;
-    QTTS_CHECK_CUDA((func_attr_once<kernel>(smem, true)));
-    QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(tiles * splits)), dim3(W * 32), smem, st, dim3(splits, 1, 1), p));
-    return QTTS_OK;
+    while (splits < kWinMaxSplits && tiles * splits * 2 <= slots && keys >= 2ll * splits * WL * 3 * 16) splits *= 2;
+    return launch_window_rows_w<FMT, D, SL, WL, 2>(p, tiles, splits, st);
 }
 
 template <int FMT, int D>
