@@ -1,0 +1,563 @@
+// Prompt chunks under a window with sinks, over the fp16 pool or the 4-bit one, on the tcgen05 pipe.
+//
+// One CTA takes 128 rows (row = query * group + head: the query heads of one KV head for consecutive
+// queries of a stream) through tiles of four 16-token blocks, only those that hold a key some row sees:
+//     S[128][64]  = Q K^T      TMEM, two buffers
+//     P           = 2^(S - m)  one thread per row; fp16 to shared memory, two buffers
+//     O[128][D]  += P V        TMEM
+// Warps 0-3 are the softmax, warps 4-7 bring K and V (one block a warp: cp.async for fp16; 4 bits are
+// turned into fp16 on the way through registers, fma(code, scale, zero) rounded once), warp 8 issues
+// the products, S one tile ahead of P V.  K and V tiles are panels of 64 channels, 128-byte rows with
+// the 128-byte swizzle; V is read in place as an MN-major operand.
+//
+// q enters as fp16 after a scaling by a power of two that brings the row's largest channel to
+// [2^11, 2^12): 2^-12 of each channel, as P's 2^-12 of each probability, a quarter of what the bf16
+// output rounds off; 4-bit values round to fp16 the same way.  Sums, maxima and O are fp32.
+//
+// Bound by: 128 x 64 exponentials a tile (512 cycles at 16 a cycle and SM) next to 512 cycles of
+// products at D = 128.  Every wait is bounded.
+#pragma once
+
+#include "attn_window.cuh"
+
+namespace qtts {
+
+constexpr int kChunkStages = 3;
+constexpr int kChunkThreads = 288;  // 4 softmax warps, 4 loading warps, 1 issuing warp
+
+template <int FMT, int D>
+struct ChunkLayout {
+    static constexpr int NW = D / 64;
+    static constexpr int PANEL = 64 * 128;            // 64 keys x 64 channels
+    static constexpr int STAGE = 2 * NW * PANEL;      // K panels, V panels
+    static constexpr int Q = 0;                       // NW panels of 128 rows
+    static constexpr int RING = Q + NW * 128 * 128;
+    static constexpr int P = RING + kChunkStages * STAGE;
+    static constexpr int SMEM = P + 2 * 128 * 128 + 1024;
+    static constexpr int PART = D + 4;                // floats per row of a partial output (bank-conflict free)
+    static_assert(128 * PART * 4 <= kChunkStages * STAGE + 2 * 128 * 128, "a partial output replaces ring and P");
+};
+
+template <int FMT, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(const WinParams p) {
+    using L = ChunkLayout<FMT, D>;
+    using G = WinChunk<FMT, D>;
+    constexpr int NW = L::NW, ST = kChunkStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t k_full[ST], v_full[ST], empty[ST], s_full[2], p_full[2], pv_done[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_lim[4][2];                                 // contexts' extremes per softmax warp
+    __shared__ __align__(16) uint8_t s_bad[ST][128];            // per key and half: V had a value that is not finite
+    __shared__ uint8_t s_here[ST][4];                           // per block: it is there and in the pool
+    __shared__ float s_part[128][2];                            // (max, sum) per row
+
+    griddep_wait();
+    griddep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t splits;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+    const uint32_t rank = cluster_ctarank();
+
+    const int tile = blockIdx.x / splits;
+    const int kvh = tile % p.kv_heads, row_tile = tile / p.kv_heads;
+    const int stream = row_tile / p.tiles, q0 = (row_tile % p.tiles) * p.qt;
+    const int nq = min(p.qt, p.S - q0), rows = nq * p.group;
+    const int row0 = stream * p.S + q0;
+    const int limit = min(p.max_ctx, p.mbps * 16);
+    const int window = p.window > 0 ? p.window : 0x7fffffff;
+    const int slot = __ldg(p.row_slot + row0);
+    const bool slot_ok = slot >= 0 && slot < p.num_slots;
+    if (!slot_ok && threadIdx.x == 0) record_error(DEV_ERR_ATTN_BOUNDS);
+
+    const int r = threadIdx.x;  // softmax threads: the row
+    int ctx = 0;
+    if (warp < 4) {
+        if (r < rows && slot_ok) ctx = min(max(__ldg(p.row_ctx + row0 + r / p.group), 0), limit);
+        int hi = ctx, lo = ctx > 0 ? ctx : 0x7fffffff;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, x));
+            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, x));
+        }
+        if (lane == 0) s_lim[warp][0] = hi, s_lim[warp][1] = lo;
+    }
+    if (warp == 8) {
+        if (lane == 0) {
+            for (int i = 0; i < ST; ++i) {
+                mbar_init(&k_full[i], 128);
+                mbar_init(&v_full[i], 128);
+                mbar_init(&empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&s_full[i], 1);
+                mbar_init(&p_full[i], 128);
+                mbar_init(&pv_done[i], 1);
+            }
+            fence_mbar_init();
+        }
+        __syncwarp();
+        tmem_alloc(&s_tmem, 256);
+        tmem_relinquish();
+    }
+    // Q: a row per softmax thread
+    float sf = 0.f;
+    if (warp < 4) {
+        const bool valid = r < rows;
+        const float4* qr = reinterpret_cast<const float4*>(
+            p.q + ((size_t)(row0 + (valid ? r / p.group : 0)) * p.num_heads + kvh * p.group + (valid ? r % p.group : 0)) * D);
+        float amax = 0.f;
+#pragma unroll 8
+        for (int c = 0; c < D / 4; ++c) {
+            const float4 u = valid ? __ldg(qr + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            amax = max_nan(max_nan(amax, max_nan(fabsf(u.x), fabsf(u.y))), max_nan(fabsf(u.z), fabsf(u.w)));
+        }
+        const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
+        const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
+        sf = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+            const float4 a = valid ? __ldg(qr + 2 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 b = valid ? __ldg(qr + 2 * c + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+            uint4 u;
+            if constexpr (FMT == kWinQ4)  // the channel order in which nibbles come apart (below)
+                u = make_uint4(pack_h2(a.x * up, b.x * up), pack_h2(a.y * up, b.y * up), pack_h2(a.z * up, b.z * up),
+                               pack_h2(a.w * up, b.w * up));
+            else
+                u = make_uint4(pack_h2(a.x * up, a.y * up), pack_h2(a.z * up, a.w * up), pack_h2(b.x * up, b.y * up),
+                               pack_h2(b.z * up, b.w * up));
+            *reinterpret_cast<uint4*>(smem + L::Q + (c >> 3) * 16384 + sw128_off(r, (c & 7) * 8)) = u;
+        }
+    }
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    int cmax = 0, cmin = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cmax = max(cmax, s_lim[i][0]), cmin = min(cmin, s_lim[i][1]);
+    const int nb_end = (cmax + 15) >> 4;
+    const int nb_sink = min((min(p.sinks, cmax) + 15) >> 4, nb_end);
+    const int first = max(nb_sink, cmax > 0 ? max(0, cmin - window) >> 4 : 0);
+    const int past_sinks = first - nb_sink;
+    const int nb = nb_sink + max(0, nb_end - first);
+    const int all_tiles = (nb + 3) >> 2;
+    const int even = all_tiles / (int)splits, rest = all_tiles % (int)splits;
+    const int t0 = (int)rank * even + min((int)rank, rest), nt = even + ((int)rank < rest);  // this CTA's tiles
+    auto first_key = [&](int pos) { return (pos < nb_sink ? pos : pos + past_sinks) * 16; };
+    auto is_whole = [&](int j0) { return j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks); };
+
+    bool ok = true;  // a wait that ran out ends the thread's loop
+    float m = -INFINITY, mu = 0.f, l = 0.f;
+    if (warp < 4) {
+        // ------------------------------------------------------------------ softmax
+        const uint32_t lanes = tmem + ((uint32_t)warp << 21);
+        for (int i = 0; i < nt && ok; ++i) {
+            const int st = i % ST, pos = (t0 + i) * 4;
+            ok = mbar_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, DEV_ERR_ATTN_WAIT) &&
+                 mbar_wait(&k_full[st], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);  // (for s_here)
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            float v[64];
+            tmem_ld32(lanes + (i & 1) * 64, reinterpret_cast<float(&)[32]>(v[0]));
+            tmem_ld32(lanes + (i & 1) * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+            const uint32_t here = *reinterpret_cast<const uint32_t*>(s_here[st]);
+            bool whole = here == 0x01010101u;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) whole = whole && is_whole(first_key(pos + b));
+            if (!whole) {
+                ok = mbar_wait(&v_full[st], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);  // (for s_bad)
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int j0 = first_key(pos + b);
+                    const bool there = (here >> (8 * b)) & 1;
+                    if (there && is_whole(j0)) continue;
+                    const uint4 bad0 = *reinterpret_cast<const uint4*>(s_bad[st] + 32 * b);
+                    const uint4 bad1 = *reinterpret_cast<const uint4*>(s_bad[st] + 32 * b + 16);
+                    const bool any = (bad0.x | bad0.y | bad0.z | bad0.w | bad1.x | bad1.y | bad1.z | bad1.w) != 0;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int j = j0 + k;
+                        const bool sees = there && j < ctx && (j >= ctx - window || j < p.sinks);
+                        if (!sees) v[16 * b + k] = -INFINITY;
+                        else if (any && *reinterpret_cast<const uint16_t*>(s_bad[st] + 32 * b + 2 * k))
+                            l = __int_as_float(0x7fffffff);  // its V was taken out: the row becomes NaN
+                    }
+                }
+            }
+            float top = v[0];
+#pragma unroll
+            for (int k = 1; k < 64; ++k) top = fmaxf(top, v[k]);
+            top *= sf;  // sf > 0; -inf stays
+            // the running maximum moves only when a score passes it by 8: P < 2^8
+            if (__any_sync(0xffffffffu, top > (m == -INFINITY ? -INFINITY : m + 8.f))) {
+                const float mn = fmaxf(m, top);
+                const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
+                m = mn;
+                mu = mn == -INFINITY ? 0.f : mn;
+                l *= corr;
+                if (i > 0) {  // O holds P V of tiles 0 .. i - 1 once the last is done
+                    ok = mbar_wait(&pv_done[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u, DEV_ERR_ATTN_WAIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        float x[16];
+                        tmem_ld16(lanes + 128 + c, x);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) x[k] *= corr;
+                        tmem_st16(lanes + 128 + c, x);
+                    }
+                }
+            }
+            float s4[4] = {0.f, 0.f, 0.f, 0.f};
+            uint8_t* pr = smem + L::P + (i & 1) * 16384;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                uint32_t u[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float a = ex2_approx(fmaf(v[8 * c + 2 * k], sf, -mu)), b = ex2_approx(fmaf(v[8 * c + 2 * k + 1], sf, -mu));
+                    s4[k] += a + b;
+                    u[k] = pack_h2(a, b);
+                }
+                *reinterpret_cast<uint4*>(pr + sw128_off(r, 8 * c)) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+            l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            fence_proxy_async_smem();
+            tc_fence_before();
+            mbar_arrive(&p_full[i & 1]);
+        }
+        if (ok && nt > 0) ok = mbar_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1u, DEV_ERR_ATTN_WAIT);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+    } else if (warp < 8) {
+        // ------------------------------------------------------------------ K and V: block `w4` of each tile
+        const int w4 = warp - 4, pt = threadIdx.x - 128, key = pt >> 1, half = pt & 1, off = key & 15;
+        const int32_t* table = p.block_table + (size_t)(slot_ok ? slot : 0) * p.mbps;
+        const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::BYTES;
+        int ids = -1;
+        auto block_id = [&](int i) {  // of this warp's block of tile i; -1: none, or outside the pool
+            if ((i & 31) == 0) {      // 32 tiles' ids, one per lane
+                const int pos = (t0 + i + lane) * 4 + w4;
+                ids = -1;
+                if (i + lane < nt && pos < nb) {
+                    ids = __ldg(table + (first_key(pos) >> 4));
+                    if (ids < 0 || ids >= p.num_blocks) {
+                        record_error(DEV_ERR_ATTN_BOUNDS);
+                        ids = -1;
+                    }
+                }
+            }
+            return __shfl_sync(0xffffffffu, ids, i & 31);
+        };
+        auto partial = [&](int i, int id) { return id < 0 || !is_whole(first_key((t0 + i) * 4 + w4)); };
+        auto seen_by_all = [&](int i, int id) {  // this thread's key
+            const int j = first_key((t0 + i) * 4 + w4) + off;
+            return id >= 0 && j < cmin && (j >= cmax - window || j < p.sinks);
+        };
+        // 16-byte piece c of this thread's half row of a tile's K (v = 0) or V
+        auto piece = [&](int st, int v, int c) {
+            const int ch = half * (D / 16) + c;  // of D / 8
+            return smem + L::RING + st * L::STAGE + (v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
+        };
+        if constexpr (FMT == kWinQ4) {
+            // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), 32 bytes of a 64-byte row
+            uint32_t kw[4 * NW], vw[4 * NW];
+            __half2 kp[NW], vp[NW];
+            int id = -1;
+            auto load = [&](int i) {
+                id = i < nt ? block_id(i) : -1;
+#pragma unroll
+                for (int c = 0; c < 4 * NW; ++c) kw[c] = vw[c] = 0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) kp[w] = vp[w] = __floats2half2_rn(0.f, 0.f);
+                if (id >= 0) {
+                    const uint8_t* kc = base + (uint64_t)(uint32_t)id * p.block_bytes;
+                    const uint8_t* vc = kc + p.v_offset;
+#pragma unroll
+                    for (int c = 0; c < NW; ++c) {
+                        const int at = off * (D / 2) + half * 16 * NW + 16 * c;
+                        *reinterpret_cast<uint4*>(kw + 4 * c) = __ldg(reinterpret_cast<const uint4*>(kc + at));
+                        *reinterpret_cast<uint4*>(vw + 4 * c) = __ldg(reinterpret_cast<const uint4*>(vc + at));
+                        const int prm = Q4Layout<D>::PARAMS + c * 64 + off * 4;
+                        kp[c] = *reinterpret_cast<const __half2*>(kc + prm);
+                        vp[c] = *reinterpret_cast<const __half2*>(vc + prm);
+                    }
+                }
+            };
+            // nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as fp16 pairs, times scale plus zero
+            auto values = [&](uint32_t x, __half2 scale, __half2 zero) {
+                const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
+                              k64 = __floats2half2_rn(-64.f, -64.f);
+                uint4 u;
+                uint32_t* o = &u.x;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t y = x >> (8 * h);
+                    const uint32_t a = (y & 0x000f000fu) | 0x64006400u, b = (y & 0x00f000f0u) | 0x64006400u;
+                    const __half2 ca = __hsub2(*reinterpret_cast<const __half2*>(&a), k1024);
+                    const __half2 cb = __hfma2(*reinterpret_cast<const __half2*>(&b), k16, k64);
+                    const __half2 va = __hfma2(ca, scale, zero), vb = __hfma2(cb, scale, zero);
+                    o[2 * h] = *reinterpret_cast<const uint32_t*>(&va);
+                    o[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&vb);
+                }
+                return u;
+            };
+            load(0);
+            for (int i = 0; i < nt; ++i) {
+                const int st = i % ST;
+                if (i >= ST) {
+                    ok = mbar_wait(&empty[st], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                if (lane == 0) s_here[st][w4] = id >= 0;
+                const bool part = partial(i, id), all = seen_by_all(i, id);
+                // word c of the half row: channels 64 w + 8 ii .. + 7, w = c % NW, ii = 4 half + c / NW
+                auto at = [&](int v, int c) {
+                    const int ii = 4 * half + c / NW;
+                    return smem + L::RING + st * L::STAGE + (v * NW + c % NW) * L::PANEL + key * 128 + ((ii ^ (key & 7)) << 4);
+                };
+#pragma unroll
+                for (int c = 0; c < 4 * NW; ++c)
+                    *reinterpret_cast<uint4*>(at(0, c)) = values(kw[c], __low2half2(kp[c % NW]), __high2half2(kp[c % NW]));
+                fence_proxy_async_smem();
+                mbar_arrive(&k_full[st]);
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < 4 * NW; ++c) {
+                    uint4 u = values(vw[c], __low2half2(vp[c % NW]), __high2half2(vp[c % NW]));
+                    if (part && !all) {
+                        uint32_t* o = &u.x;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, bad = true;
+                            if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, bad = true;
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(at(1, c)) = u;
+                }
+                if (part) s_bad[st][pt] = bad;
+                load(i + 1);
+                fence_proxy_async_smem();
+                mbar_arrive(&v_full[st]);
+            }
+        } else {
+            auto issue = [&](int i) {  // tile i's copies, K and V a group each
+                const int st = i % ST, id = i < nt ? block_id(i) : -1;
+                if (i < nt && lane == 0) s_here[st][w4] = id >= 0;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    if (i < nt) {
+                        const uint8_t* src = base + (uint64_t)(uint32_t)max(id, 0) * p.block_bytes + (v ? p.v_offset : 0) +
+                                             off * (2 * D) + half * D;
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            if (id >= 0) cp_async16(smem_u32(piece(st, v, c)), src + 16 * c);
+                            else *reinterpret_cast<uint4*>(piece(st, v, c)) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    cp_async_commit();
+                }
+                return id;
+            };
+            int id = issue(0), id1 = issue(1);
+            for (int i = 0; i < nt; ++i) {
+                const int st = i % ST;
+                cp_async_wait<3>();
+                fence_proxy_async_smem();
+                mbar_arrive(&k_full[st]);
+                cp_async_wait<2>();
+                if (partial(i, id)) {
+                    bool bad = false;
+                    if (!seen_by_all(i, id)) {
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint4 u = *reinterpret_cast<const uint4*>(piece(st, 1, c));
+                            uint32_t* o = &u.x;
+                            bool here = false;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, here = true;
+                                if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, here = true;
+                            }
+                            if (here) *reinterpret_cast<uint4*>(piece(st, 1, c)) = u;
+                            bad |= here;
+                        }
+                    }
+                    s_bad[st][pt] = bad;
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&v_full[st]);
+                // tile i + 2 takes the stage of i - 1, whose products need nothing past tile i
+                if (i + 2 < nt && i >= 1) {
+                    ok = mbar_wait(&empty[(i + 2) % ST], (uint32_t)((i + 2) / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                id = id1;
+                id1 = issue(i + 2);
+            }
+            cp_async_wait<0>();
+        }
+    } else if (lane == 0) {
+        // ------------------------------------------------------------------ products
+        const uint32_t idesc_s = make_idesc_f16(128, 64), idesc_o = make_idesc_f16(128, D) | (1u << 16);  // V is MN-major
+        const uint32_t q_at = smem_u32(smem + L::Q);
+        auto issue_s = [&](int i) {
+            if (!mbar_wait(&k_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT)) return false;
+            tc_fence_after();
+            const uint32_t k_at = smem_u32(smem + L::RING + (i % ST) * L::STAGE);
+#pragma unroll
+            for (int kk = 0; kk < 4 * NW; ++kk)
+                umma_bf16(tmem + (i & 1) * 64, make_sw128_desc(q_at + (kk >> 2) * 16384) + 2 * (kk & 3),
+                          make_sw128_desc(k_at + (kk >> 2) * L::PANEL) + 2 * (kk & 3), idesc_s, kk ? 1u : 0u);
+            umma_commit(&s_full[i & 1]);
+            return true;
+        };
+        if (nt > 0) ok = issue_s(0);
+        for (int i = 0; i < nt && ok; ++i) {
+            if (i + 1 < nt) ok = issue_s(i + 1);
+            ok = ok && mbar_wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u, DEV_ERR_ATTN_WAIT);
+            ok = ok && mbar_wait(&v_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t p_at = smem_u32(smem + L::P + (i & 1) * 16384);
+            const uint32_t v_at = smem_u32(smem + L::RING + (i % ST) * L::STAGE + NW * L::PANEL);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                umma_bf16(tmem + 128u, make_sw128_desc(p_at) + 2 * kk, make_sw128_mn_desc(v_at + kk * 2048, L::PANEL), idesc_o,
+                          (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&empty[i % ST]);
+            umma_commit(&pv_done[i & 1]);
+        }
+        if (!ok) {  // every product issued so far ends before TMEM is given back
+            __shared__ uint64_t drain;
+            mbar_init(&drain, 1);
+            fence_mbar_init();
+            umma_commit(&drain);
+            mbar_wait(&drain, 0, DEV_ERR_DRAIN);
+        }
+    }
+
+    // ---------------------------------------------------------------------- out
+    if (ctx == 0) l = 0.f;  // a row without keys in a tile of rows that have some
+    float* part = reinterpret_cast<float*>(smem + L::RING);
+    auto out_at = [&](int row, int d) {
+        return ((size_t)(row0 + row / p.group) * p.num_heads + kvh * p.group + row % p.group) * D + d;
+    };
+    __syncwarp();
+    if (warp < 4) {
+        const uint32_t lanes = tmem + ((uint32_t)warp << 21) + 128;
+        const bool sum = ok && nt > 0 && l != 0.f;  // else zeros (NaN counts as a sum)
+        const float inv = sum ? 1.f / l : 0.f;
+        s_part[r][0] = m;
+        s_part[r][1] = ok ? l : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+            float x[16], y[16];
+            tmem_ld16(lanes + c, x);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                // 4 bits: position 8 n + k of V holds channel 8 n + k / 2 + 4 (k % 2)
+                const int ch = FMT == kWinQ4 ? (k & 8) + ((k & 7) >> 1) + 4 * (k & 1) : k;
+                y[ch] = sum ? (splits == 1 ? x[k] * inv : x[k]) : 0.f;
+            }
+            if (splits > 1) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<float4*>(part + r * L::PART + c + 4 * k) =
+                        make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+            } else if (r < rows) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * k], y[2 * k + 1]);
+                    const float2 f = __bfloat1622float2(h);
+                    const __nv_bfloat162 g = __floats2bfloat162_rn(y[2 * k] - f.x, y[2 * k + 1] - f.y);
+                    hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[k] = *reinterpret_cast<const uint32_t*>(&g);
+                }
+                uint4* o = reinterpret_cast<uint4*>(p.out + out_at(r, c));
+                o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                if (p.out_lo) {
+                    uint4* ol = reinterpret_cast<uint4*>(p.out_lo + out_at(r, c));
+                    ol[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    ol[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) tmem_dealloc(tmem, 256);
+    if (splits == 1) return;
+    cluster_sync();
+    for (int j = (int)rank * (kChunkThreads / 32) + warp; j < rows * (D / 32); j += (int)splits * (kChunkThreads / 32)) {
+        const int row = j / (D / 32), d = (j % (D / 32)) * 32 + lane;
+        float mc = -INFINITY, lc = 0.f;
+        if (lane < (int)splits) {
+            mc = ld_dsmem_now(map_to_rank(smem_u32(&s_part[row][0]), lane));
+            lc = ld_dsmem_now(map_to_rank(smem_u32(&s_part[row][1]), lane));
+        }
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < (int)splits) v[c] = ld_dsmem_now(map_to_rank(smem_u32(part + row * L::PART + d), c));
+        const float mx = warp_max(mc);
+        const float f = mc == -INFINITY ? 0.f : ex2_approx(mc - mx);
+        const float sum = warp_sum(mc == -INFINITY && lc != 0.f ? lc : lc * f);
+        float acc = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float fc = __shfl_sync(0xffffffffu, f, c);
+            if (c < (int)splits && fc != 0.f) acc = fmaf(v[c], fc, acc);
+        }
+        const float x = sum == 0.f ? 0.f : acc / sum;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(x);
+        p.out[out_at(row, d)] = hi;
+        if (p.out_lo) p.out_lo[out_at(row, d)] = __float2bfloat16_rn(x - __bfloat162float(hi));
+    }
+    cluster_sync();  // no CTA leaves while another reads its shared memory
+}
+
+// Whether rows go through 128-row tiles.
+inline bool use_chunk_kernel(const WinParams& p) {
+    if (p.S < 2 || p.group > 128) return false;
+    if (((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_lo)) & 15) != 0) return false;
+    return p.S * p.group >= 32;
+}
+
+template <int FMT, int D>
+inline int launch_chunk_attention(WinParams p, cudaStream_t st) {
+    using L = ChunkLayout<FMT, D>;
+    using G = WinChunk<FMT, D>;
+    p.qt = 128 / p.group < p.S ? 128 / p.group : p.S;
+    p.tiles = ceil_div(p.S, p.qt);
+    const long long block_bytes = (long long)p.num_layers * 2 * p.kv_heads * G::BYTES;
+    QTTS_REQUIRE(block_bytes < (1ll << 31), "paged attention: %lld bytes per block", block_bytes);
+    p.block_bytes = (uint32_t)block_bytes;
+    p.v_offset = (uint32_t)(p.kv_heads * G::BYTES);
+    const long long tiles = (long long)(p.R / p.S) * p.tiles * p.kv_heads;
+    QTTS_REQUIRE(tiles * 8 < (1ll << 31), "paged attention: %lld tiles", tiles);
+    const int limit = p.max_ctx < p.mbps * 16 ? p.max_ctx : p.mbps * 16;
+    long long keys = limit;
+    if (p.window > 0 && (long long)p.window + p.sinks + p.qt + 32 < keys) keys = (long long)p.window + p.sinks + p.qt + 32;
+    // a cluster shares the keys of a tile while all CTAs have an SM of their own and two tiles each
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= num_sms() && keys >= 2ll * splits * 2 * 64) splits *= 2;
+    constexpr auto kernel = paged_attn_chunk_kernel<FMT, D>;
+    QTTS_CHECK_CUDA((func_attr_once<kernel>(L::SMEM)));
+    QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(tiles * splits)), dim3(kChunkThreads), L::SMEM, st, dim3(splits, 1, 1), p));
+    return QTTS_OK;
+}
+
+}  // namespace qtts

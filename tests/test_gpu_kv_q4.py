@@ -8,7 +8,11 @@ halves (2^-17): without q's own rounding a score is off by less than 2^-14 for t
 q is two fp16 halves (2^-22, covered by that) over the fp16 pool.  Over the 4-bit pool it is a 16-bit
 fixed-point number, each channel off by at most max|q| / 65278 (half a unit): a score by at most
 d = max|q| / 65278 sum|k| / sqrt(D), a probability by a factor within exp(+-2 d) (numerator and sum), an
-output by (exp(2 d) - 1) max|v| more."""
+output by (exp(2 d) - 1) max|v| more.
+Chunks of rows go through fp16 tiles: q and P round to fp16 (2^-11), and so do 4-bit values: d = 2^-11
+sum|q k| / sqrt(D) (twice that at 4 bits), and 2^-11 max|v| for P (once more at 4 bits).  Those bounds let all
+roundings conspire; as they are independent, the root mean square over a row is held to twice its
+expectation's bound as well: (d2 + 2^-11) rms(v) with d2 = 2^-11 |q| max|k| / D (times sqrt 2 at 4 bits)."""
 
 
 import numpy as np
@@ -254,12 +258,30 @@ def _attend(fmt, *a, window=0, sinks=0, **kw):
     return ops.paged_attention_q4(*a, window=window, sinks=sinks, **kw)
 
 
-def _tolerance(fmt, q, kv):
+def _is_chunk(S, Hq, H):
+    return S > 1 and S * Hq // H >= 32
+
+
+def _tolerance(fmt, q, kv, chunk=False):
     """Absolute tolerance of out + out_lo for one row (see the module's docstring)."""
     if not kv.size:
         return 0.0
-    d = np.abs(q).max() / 65278 * np.abs(kv[0]).sum(-1).max() / np.sqrt(q.shape[-1]) if fmt == "q4" else 0.0
-    return (2.0 ** -12 + np.expm1(2 * d)) * np.abs(kv[1]).max()
+    top = np.abs(kv[1]).max()
+    group, D = len(q) // len(kv[0]), q.shape[-1]
+    if chunk:
+        q4 = fmt == "q4"
+        d = 2.0 ** -11 * (1 + q4) * max((np.abs(kv[0][h // group]) @ np.abs(q[h])).max() for h in range(len(q))) / np.sqrt(D)
+        return (2.0 ** -12 + np.expm1(2 * d) + 2.0 ** -11 * (1 + q4)) * top
+    d = np.abs(q).max() / 65278 * np.abs(kv[0]).sum(-1).max() / np.sqrt(D) if fmt == "q4" else 0.0
+    return (2.0 ** -12 + np.expm1(2 * d)) * top
+
+
+def _rms_tolerance(fmt, q, kv):
+    """Root mean square over a row of a chunk (see the module's docstring)."""
+    if not kv.size:
+        return 0.0
+    d2 = 2.0 ** -11 * np.linalg.norm(q, axis=-1).max() * np.linalg.norm(kv[0], axis=-1).max() / q.shape[-1]
+    return 2 * (d2 * (np.sqrt(2) if fmt == "q4" else 1) + 2.0 ** -11) * np.sqrt((kv[1] ** 2).mean())
 
 
 def _run_case(fmt, Hq, H, D, ctxs, S, window, sinks, seed=0, max_ctx=None, poison=None, qscale=1.0):
@@ -291,8 +313,10 @@ def _run_case(fmt, Hq, H, D, ctxs, S, window, sinks, seed=0, max_ctx=None, poiso
         for t in range(S):
             r = b * S + t
             want = O.attention(q[r].numpy(), kv[0], kv[1], min(int(row_ctx[r]), limit), window, sinks)
-            tol = _tolerance(fmt, q[r].numpy(), kv)
+            tol = _tolerance(fmt, q[r].numpy(), kv, _is_chunk(S, Hq, H))
             assert np.abs(got[r] - want).max() <= tol, (r, np.abs(got[r] - want).max(), tol)
+            if _is_chunk(S, Hq, H):
+                assert np.sqrt(((got[r] - want) ** 2).mean()) <= _rms_tolerance(fmt, q[r].numpy(), kv), r
     return out
 
 
@@ -407,7 +431,7 @@ def test_nan_key_inside_a_chunk_reaches_later_rows_only(fmt, S):
             want = O.attention(q[r].numpy(), kv[0], kv[1], int(ctxs[r]))
             # bf16 output alone: half a unit (2^-8 of the value), then the tolerance of the pair
             err = np.abs(out[r].double().numpy().reshape(-1) - want)
-            assert (err <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[r].numpy(), kv)).all()
+            assert (err <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[r].numpy(), kv, _is_chunk(S, 4, H))).all()
 
 
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
