@@ -22,27 +22,30 @@
 
 namespace qtts {
 
-constexpr int kChunkStages = 3;
 constexpr int kChunkThreads = 288;  // 4 softmax warps, 4 loading warps, 1 issuing warp
 
 template <int FMT, int D>
 struct ChunkLayout {
     static constexpr int NW = D / 64;
+    static constexpr int ST = FMT == kWinQ4 ? 3 : 4;  // stages of fp16 tiles
+    static constexpr int RAW = FMT == kWinQ4 ? 4 : 0; // tiles of codes on their way (cp.async), before they are turned into fp16
     static constexpr int PANEL = 64 * 128;            // 64 keys x 64 channels
     static constexpr int STAGE = 2 * NW * PANEL;      // K panels, V panels
     static constexpr int Q = 0;                       // NW panels of 128 rows
     static constexpr int RING = Q + NW * 128 * 128;
-    static constexpr int P = RING + kChunkStages * STAGE;
-    static constexpr int SMEM = P + 2 * 128 * 128 + 1024;
-    static constexpr int PART = D + 4;                // floats per row of a partial output (bank-conflict free)
-    static_assert(128 * PART * 4 <= kChunkStages * STAGE + 2 * 128 * 128, "a partial output replaces ring and P");
+    static constexpr int P = RING + ST * STAGE;
+    static constexpr int CODES = P + 2 * 128 * 128;   // [warp][RAW][K, V] chunks
+    static constexpr int SMEM = CODES + 4 * RAW * 2 * WinChunk<FMT, D>::BYTES + 1024;
+    static constexpr int PART = D + 4;                // floats per row of a partial output (no bank met twice)
+    static_assert(128 * PART * 4 <= ST * STAGE + 2 * 128 * 128, "a partial output replaces ring and P");
+    static_assert(SMEM + 4096 <= 227 * 1024, "tile exceeds shared memory");
 };
 
 template <int FMT, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(const WinParams p) {
     using L = ChunkLayout<FMT, D>;
     using G = WinChunk<FMT, D>;
-    constexpr int NW = L::NW, ST = kChunkStages;
+    constexpr int NW = L::NW, ST = L::ST;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t k_full[ST], v_full[ST], empty[ST], s_full[2], p_full[2], pv_done[2];
@@ -51,6 +54,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     __shared__ __align__(16) uint8_t s_bad[ST][128];            // per key and half: V had a value that is not finite
     __shared__ uint8_t s_here[ST][4];                           // per block: it is there and in the pool
     __shared__ float s_part[128][2];                            // (max, sum) per row
+    __shared__ float s_sf[128];                                 // accumulator -> log2 units, per row
 
     griddep_wait();
     griddep_launch();
@@ -64,6 +68,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     const int stream = row_tile / p.tiles, q0 = (row_tile % p.tiles) * p.qt;
     const int nq = min(p.qt, p.S - q0), rows = nq * p.group;
     const int row0 = stream * p.S + q0;
+    const size_t head0 = (size_t)row0 * p.num_heads + kvh * p.group;  // q and out row (head) of tile row 0
+    auto head_row = [&](int row) { return head0 + (uint32_t)(p.by_group.div(row) * (p.num_heads - p.group) + row); };
     const int limit = min(p.max_ctx, p.mbps * 16);
     const int window = p.window > 0 ? p.window : 0x7fffffff;
     const int slot = __ldg(p.row_slot + row0);
@@ -73,7 +79,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     const int r = threadIdx.x;  // softmax threads: the row
     int ctx = 0;
     if (warp < 4) {
-        if (r < rows && slot_ok) ctx = min(max(__ldg(p.row_ctx + row0 + r / p.group), 0), limit);
+        if (r < rows && slot_ok) ctx = min(max(__ldg(p.row_ctx + row0 + p.by_group.div(r)), 0), limit);
         int hi = ctx, lo = ctx > 0 ? ctx : 0x7fffffff;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) {
@@ -100,33 +106,44 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         tmem_alloc(&s_tmem, 256);
         tmem_relinquish();
     }
-    // Q: a row per softmax thread
-    float sf = 0.f;
-    if (warp < 4) {
-        const bool valid = r < rows;
-        const float4* qr = reinterpret_cast<const float4*>(
-            p.q + ((size_t)(row0 + (valid ? r / p.group : 0)) * p.num_heads + kvh * p.group + (valid ? r % p.group : 0)) * D);
-        float amax = 0.f;
-#pragma unroll 8
-        for (int c = 0; c < D / 4; ++c) {
-            const float4 u = valid ? __ldg(qr + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            amax = max_nan(max_nan(amax, max_nan(fabsf(u.x), fabsf(u.y))), max_nan(fabsf(u.z), fabsf(u.w)));
-        }
-        const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
-        const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
-        sf = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-            const float4 a = valid ? __ldg(qr + 2 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float4 b = valid ? __ldg(qr + 2 * c + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
-            uint4 u;
-            if constexpr (FMT == kWinQ4)  // the channel order in which nibbles come apart (below)
-                u = make_uint4(pack_h2(a.x * up, b.x * up), pack_h2(a.y * up, b.y * up), pack_h2(a.z * up, b.z * up),
-                               pack_h2(a.w * up, b.w * up));
-            else
-                u = make_uint4(pack_h2(a.x * up, a.y * up), pack_h2(a.z * up, a.w * up), pack_h2(b.x * up, b.y * up),
-                               pack_h2(b.z * up, b.w * up));
-            *reinterpret_cast<uint4*>(smem + L::Q + (c >> 3) * 16384 + sw128_off(r, (c & 7) * 8)) = u;
+    // Q: warps 0-7 take 16 rows each, a row (D = 64: two) at a time, four channels a lane, the next
+    // four steps' loads under way
+    if (warp < 8) {
+        constexpr int RPI = 128 / D, LPR = 32 / RPI;  // rows per step, lanes per row
+        const int c = lane % LPR, first_row = warp * 16 + lane / LPR;
+        auto fetch = [&](int k) {
+            const int row = first_row + k * RPI;
+            return row < rows && k * RPI < 16 ? __ldg(reinterpret_cast<const float4*>(p.q + head_row(row) * D) + c)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        float4 u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = fetch(k);
+#pragma unroll 1
+        for (int k0 = 0; k0 < 16 / RPI; k0 += 4) {
+            float4 next[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) next[k] = fetch(k0 + 4 + k);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = first_row + (k0 + k) * RPI;
+                float amax = max_nan(max_nan(fabsf(u[k].x), fabsf(u[k].y)), max_nan(fabsf(u[k].z), fabsf(u[k].w)));
+#pragma unroll
+                for (int x = 1; x < LPR; x <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, x));
+                const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
+                const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
+                uint2 h = make_uint2(pack_h2(u[k].x * up, u[k].y * up), pack_h2(u[k].z * up, u[k].w * up));
+                if constexpr (FMT == kWinQ4) {
+                    // the channel order in which nibbles come apart (below): 0 4 1 5 2 6 3 7 of each eight.
+                    // An even lane holds 0 1 2 3 and makes 0 4 1 5, the odd one beside it 4 5 6 7 and 2 6 3 7
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? h.x : h.y, 1);
+                    h = lane & 1 ? make_uint2(prmt(other, h.y, 0x5410), prmt(other, h.y, 0x7632))
+                                 : make_uint2(prmt(h.x, other, 0x5410), prmt(h.x, other, 0x7632));
+                }
+                *reinterpret_cast<uint2*>(smem + L::Q + (c >> 4) * 16384 + sw128_off(row, (c & 15) * 4)) = h;
+                if (c == 0) s_sf[row] = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
+                u[k] = next[k];
+            }
         }
     }
     fence_proxy_async_smem();
@@ -150,6 +167,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     auto is_whole = [&](int j0) { return j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks); };
 
     bool ok = true;  // a wait that ran out ends the thread's loop
+    const float sf = s_sf[r & 127];
     float m = -INFINITY, mu = 0.f, l = 0.f;
     if (warp < 4) {
         // ------------------------------------------------------------------ softmax
@@ -177,23 +195,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     const int j0 = first_key(pos + b);
                     const bool there = (here >> (8 * b)) & 1;
                     if (there && is_whole(j0)) continue;
+                    // bit k: the row sees key j0 + k
+                    auto below = [&](int j) { return (1u << min(max(j - j0, 0), 16)) - 1u; };
+                    uint32_t sees = below(ctx) & (~below(max(ctx - window, 0)) | below(p.sinks));
+                    if (!there) sees = 0;
                     const uint4 bad0 = *reinterpret_cast<const uint4*>(s_bad[st] + 32 * b);
                     const uint4 bad1 = *reinterpret_cast<const uint4*>(s_bad[st] + 32 * b + 16);
-                    const bool any = (bad0.x | bad0.y | bad0.z | bad0.w | bad1.x | bad1.y | bad1.z | bad1.w) != 0;
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const int j = j0 + k;
-                        const bool sees = there && j < ctx && (j >= ctx - window || j < p.sinks);
-                        if (!sees) v[16 * b + k] = -INFINITY;
-                        else if (any && *reinterpret_cast<const uint16_t*>(s_bad[st] + 32 * b + 2 * k))
-                            l = __int_as_float(0x7fffffff);  // its V was taken out: the row becomes NaN
+                    if ((bad0.x | bad0.y | bad0.z | bad0.w | bad1.x | bad1.y | bad1.z | bad1.w) != 0) {
+                        for (int k = 0; k < 16; ++k)  // its V was taken out: the row becomes NaN
+                            if (((sees >> k) & 1) && *reinterpret_cast<const uint16_t*>(s_bad[st] + 32 * b + 2 * k))
+                                l = __int_as_float(0x7fffffff);
                     }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (!(sees & (1u << k))) v[16 * b + k] = -INFINITY;
                 }
             }
-            float top = v[0];
+            float t8[8];
 #pragma unroll
-            for (int k = 1; k < 64; ++k) top = fmaxf(top, v[k]);
-            top *= sf;  // sf > 0; -inf stays
+            for (int k = 0; k < 8; ++k) t8[k] = v[k];
+#pragma unroll
+            for (int k = 8; k < 64; ++k) t8[k & 7] = fmaxf(t8[k & 7], v[k]);
+            // sf > 0; -inf stays
+            const float top = sf * fmaxf(fmaxf(fmaxf(t8[0], t8[1]), fmaxf(t8[2], t8[3])),
+                                         fmaxf(fmaxf(t8[4], t8[5]), fmaxf(t8[6], t8[7])));
             // the running maximum moves only when a score passes it by 8: P < 2^8
             if (__any_sync(0xffffffffu, top > (m == -INFINITY ? -INFINITY : m + 8.f))) {
                 const float mn = fmaxf(m, top);
@@ -268,30 +293,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             return smem + L::RING + st * L::STAGE + (v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
         };
         if constexpr (FMT == kWinQ4) {
-            // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), 32 bytes of a 64-byte row
-            uint32_t kw[4 * NW], vw[4 * NW];
-            __half2 kp[NW], vp[NW];
-            int id = -1;
-            auto load = [&](int i) {
-                id = i < nt ? block_id(i) : -1;
-#pragma unroll
-                for (int c = 0; c < 4 * NW; ++c) kw[c] = vw[c] = 0;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) kp[w] = vp[w] = __floats2half2_rn(0.f, 0.f);
+            // codes: this warp's chunks through its own ring, RAW - 1 tiles ahead
+            const uint32_t raw = smem_u32(smem + L::CODES) + w4 * L::RAW * 2 * G::BYTES;
+            uint32_t valid = 0;  // bit i % 32: tile i's block is there
+            auto fetch = [&](int i) {
+                const int id = i < nt ? block_id(i) : -1;
+                valid = id >= 0 ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
                 if (id >= 0) {
-                    const uint8_t* kc = base + (uint64_t)(uint32_t)id * p.block_bytes;
-                    const uint8_t* vc = kc + p.v_offset;
+                    const uint8_t* src = base + (uint64_t)(uint32_t)id * p.block_bytes;
+                    const uint32_t dst = raw + (i % L::RAW) * 2 * G::BYTES;
 #pragma unroll
-                    for (int c = 0; c < NW; ++c) {
-                        const int at = off * (D / 2) + half * 16 * NW + 16 * c;
-                        *reinterpret_cast<uint4*>(kw + 4 * c) = __ldg(reinterpret_cast<const uint4*>(kc + at));
-                        *reinterpret_cast<uint4*>(vw + 4 * c) = __ldg(reinterpret_cast<const uint4*>(vc + at));
-                        const int prm = Q4Layout<D>::PARAMS + c * 64 + off * 4;
-                        kp[c] = *reinterpret_cast<const __half2*>(kc + prm);
-                        vp[c] = *reinterpret_cast<const __half2*>(vc + prm);
-                    }
+                    for (int v = 0; v < 2; ++v)
+#pragma unroll
+                        for (int c = 0; c < G::BYTES / 16; c += 32)
+                            if (c + lane < G::BYTES / 16)
+                                cp_async16(dst + v * G::BYTES + (c + lane) * 16, src + v * p.v_offset + (c + lane) * 16);
                 }
+                cp_async_commit();
             };
+#pragma unroll
+            for (int i = 0; i < L::RAW - 1; ++i) fetch(i);
             // nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as fp16 pairs, times scale plus zero
             auto values = [&](uint32_t x, __half2 scale, __half2 zero) {
                 const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
@@ -310,9 +331,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 return u;
             };
-            load(0);
             for (int i = 0; i < nt; ++i) {
                 const int st = i % ST;
+                cp_async_wait<L::RAW - 2>();
+                __syncwarp();  // tile i's codes are there, and every lane is done with the ring's slot of tile i - 1
+                fetch(i + L::RAW - 1);
+                const int id = (valid >> (i & 31)) & 1 ? 0 : -1;
+                // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), of a row of 4 D / 32
+                uint32_t kw[NW][4] = {}, vw[NW][4] = {};
+                float2 kp[NW], vp[NW];
+#pragma unroll
+                for (int c = 0; c < NW; ++c) kp[c] = vp[c] = make_float2(0.f, 0.f);
+                if (id >= 0) {
+                    const uint32_t at = raw + (i % L::RAW) * 2 * G::BYTES;
+#pragma unroll
+                    for (int c = 0; c < NW; ++c) {
+                        lds_words(kw[c], at + off * (D / 2) + half * 16 * NW + 16 * c);
+                        lds_words(vw[c], at + G::BYTES + off * (D / 2) + half * 16 * NW + 16 * c);
+                        kp[c] = lds_half2(at + Q4Layout<D>::PARAMS + c * 64 + off * 4);
+                        vp[c] = lds_half2(at + G::BYTES + Q4Layout<D>::PARAMS + c * 64 + off * 4);
+                    }
+                }
                 if (i >= ST) {
                     ok = mbar_wait(&empty[st], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
                     ok = __all_sync(0xffffffffu, ok);
@@ -327,13 +366,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 };
 #pragma unroll
                 for (int c = 0; c < 4 * NW; ++c)
-                    *reinterpret_cast<uint4*>(at(0, c)) = values(kw[c], __low2half2(kp[c % NW]), __high2half2(kp[c % NW]));
+                    *reinterpret_cast<uint4*>(at(0, c)) = values(kw[c >> 2][c & 3], __float2half2_rn(kp[c % NW].x), __float2half2_rn(kp[c % NW].y));
                 fence_proxy_async_smem();
                 mbar_arrive(&k_full[st]);
                 bool bad = false;
 #pragma unroll
                 for (int c = 0; c < 4 * NW; ++c) {
-                    uint4 u = values(vw[c], __low2half2(vp[c % NW]), __high2half2(vp[c % NW]));
+                    uint4 u = values(vw[c >> 2][c & 3], __float2half2_rn(vp[c % NW].x), __float2half2_rn(vp[c % NW].y));
                     if (part && !all) {
                         uint32_t* o = &u.x;
 #pragma unroll
@@ -345,10 +384,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     *reinterpret_cast<uint4*>(at(1, c)) = u;
                 }
                 if (part) s_bad[st][pt] = bad;
-                load(i + 1);
                 fence_proxy_async_smem();
                 mbar_arrive(&v_full[st]);
             }
+            cp_async_wait<0>();
         } else {
             auto issue = [&](int i) {  // tile i's copies, K and V a group each
                 const int st = i % ST, id = i < nt ? block_id(i) : -1;
@@ -368,13 +407,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 return id;
             };
-            int id = issue(0), id1 = issue(1);
+            uint32_t valid = 0;  // bit i % 32: tile i's block is there
+            auto start = [&](int i) {
+                const bool in = issue(i) >= 0;
+                valid = in ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
+            };
+#pragma unroll
+            for (int i = 0; i < ST - 1; ++i) start(i);
             for (int i = 0; i < nt; ++i) {
-                const int st = i % ST;
-                cp_async_wait<3>();
+                const int st = i % ST, id = (valid >> (i & 31)) & 1 ? 0 : -1;
+                cp_async_wait<2 * (ST - 1) - 1>();
                 fence_proxy_async_smem();
                 mbar_arrive(&k_full[st]);
-                cp_async_wait<2>();
+                cp_async_wait<2 * (ST - 1) - 2>();
                 if (partial(i, id)) {
                     bool bad = false;
                     if (!seen_by_all(i, id)) {
@@ -396,14 +441,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(&v_full[st]);
-                // tile i + 2 takes the stage of i - 1, whose products need nothing past tile i
-                if (i + 2 < nt && i >= 1) {
-                    ok = mbar_wait(&empty[(i + 2) % ST], (uint32_t)((i + 2) / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
+                // the next tile takes the stage of i - 1, whose products need nothing past tile i
+                const int next = i + ST - 1;
+                if (next < nt && i >= 1) {
+                    ok = mbar_wait(&empty[next % ST], (uint32_t)(next / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
-                id = id1;
-                id1 = issue(i + 2);
+                start(next);
             }
             cp_async_wait<0>();
         }
@@ -450,9 +495,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     // ---------------------------------------------------------------------- out
     if (ctx == 0) l = 0.f;  // a row without keys in a tile of rows that have some
     float* part = reinterpret_cast<float*>(smem + L::RING);
-    auto out_at = [&](int row, int d) {
-        return ((size_t)(row0 + row / p.group) * p.num_heads + kvh * p.group + row % p.group) * D + d;
-    };
+    auto out_at = [&](int row, int d) { return head_row(row) * D + d; };
     __syncwarp();
     if (warp < 4) {
         const uint32_t lanes = tmem + ((uint32_t)warp << 21) + 128;
@@ -460,6 +503,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         const float inv = sum ? 1.f / l : 0.f;
         s_part[r][0] = m;
         s_part[r][1] = ok ? l : 0.f;
+        constexpr int ROWB = 2 * D + 16;  // bytes of a staged output row
+        uint8_t* rows_at = smem + L::RING + warp * 64 * ROWB;
+        static_assert(4 * 64 * ROWB <= ST * L::STAGE, "staged output rows replace the ring");
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
             float x[16], y[16];
@@ -475,7 +521,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 for (int k = 0; k < 4; ++k)
                     *reinterpret_cast<float4*>(part + r * L::PART + c + 4 * k) =
                         make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
-            } else if (r < rows) {
+            } else {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -485,14 +531,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     hi[k] = *reinterpret_cast<const uint32_t*>(&h);
                     lo[k] = *reinterpret_cast<const uint32_t*>(&g);
                 }
-                uint4* o = reinterpret_cast<uint4*>(p.out + out_at(r, c));
+                uint4* o = reinterpret_cast<uint4*>(rows_at + lane * ROWB + 2 * c);
                 o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
                 if (p.out_lo) {
-                    uint4* ol = reinterpret_cast<uint4*>(p.out_lo + out_at(r, c));
+                    uint4* ol = reinterpret_cast<uint4*>(rows_at + 32 * ROWB + lane * ROWB + 2 * c);
                     ol[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     ol[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
                 }
+            }
+        }
+        if (splits == 1) {
+            // a warp's 32 rows leave through shared memory, so that its stores are whole rows
+            __syncwarp();
+#pragma unroll 4
+            for (int k = lane; k < 32 * (D / 8); k += 32) {
+                const int row = k / (D / 8), c = k % (D / 8);
+                if (warp * 32 + row >= rows) break;
+                const size_t at = out_at(warp * 32 + row, 8 * c);
+                *reinterpret_cast<uint4*>(p.out + at) = *reinterpret_cast<const uint4*>(rows_at + row * ROWB + 16 * c);
+                if (p.out_lo)
+                    *reinterpret_cast<uint4*>(p.out_lo + at) =
+                        *reinterpret_cast<const uint4*>(rows_at + 32 * ROWB + row * ROWB + 16 * c);
             }
         }
     }

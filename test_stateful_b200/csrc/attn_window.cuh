@@ -48,6 +48,7 @@ struct WinParams {
     int R, S;               // rows; consecutive rows that belong to one stream
     int num_heads, kv_heads;
     int group;              // query heads per KV head
+    FastDiv by_group;
     int head_tiles;         // tiles a KV head's query heads are cut into
     int qt, tiles;          // queries per tile, tiles per stream
     int layer, num_layers, num_blocks, num_slots, mbps;

@@ -94,6 +94,7 @@ static int window_attention(const char* what, int fmt, const void* q, int R, int
     p.num_heads = num_heads;
     p.kv_heads = kv_heads;
     p.group = num_heads / kv_heads;
+    p.by_group = make_fastdiv((uint32_t)p.group);
     p.layer = layer;
     p.num_layers = num_layers;
     p.num_blocks = num_blocks;
