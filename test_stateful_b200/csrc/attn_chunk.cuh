@@ -5,8 +5,8 @@
 //     S[128][64]  = Q K^T      TMEM, two buffers
 //     P           = 2^(S - m)  one thread per row; fp16 to shared memory, two buffers
 //     O[128][D]  += P V        TMEM
-// Warps 0-3 are the softmax, warps 4-7 bring K and V (one block a warp: cp.async for fp16; 4 bits are
-// turned into fp16 on the way through registers, fma(code, scale, zero) rounded once), warp 8 issues
+// Warps 0-3 are the softmax, warps 4-7 bring K and 8-11 V (one block a warp: cp.async for fp16; 4 bits
+// are turned into fp16 on the way through registers, fma(code, scale, zero) rounded once), warp 12 issues
 // the products, S one tile ahead of P V.  K and V tiles are panels of 64 channels, 128-byte rows with
 // the 128-byte swizzle; V is read in place as an MN-major operand.
 //
@@ -22,7 +22,7 @@
 
 namespace qtts {
 
-constexpr int kChunkThreads = 288;  // 4 softmax warps, 4 loading warps, 1 issuing warp
+constexpr int kChunkThreads = 416;  // 4 softmax warps, 4 for K, 4 for V, 1 issuing warp
 
 template <int FMT, int D>
 struct ChunkLayout {
@@ -34,7 +34,7 @@ struct ChunkLayout {
     static constexpr int Q = 0;                       // NW panels of 128 rows
     static constexpr int RING = Q + NW * 128 * 128;
     static constexpr int P = RING + ST * STAGE;
-    static constexpr int CODES = P + 2 * 128 * 128;   // [warp][RAW][K, V] chunks
+    static constexpr int CODES = P + 2 * 128 * 128;   // [K, V][warp][RAW] chunks
     static constexpr int SMEM = CODES + 4 * RAW * 2 * WinChunk<FMT, D>::BYTES + 1024;
     static constexpr int PART = D + 4;                // floats per row of a partial output (no bank met twice)
     static_assert(128 * PART * 4 <= ST * STAGE + 2 * 128 * 128, "a partial output replaces ring and P");
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         }
         if (lane == 0) s_lim[warp][0] = hi, s_lim[warp][1] = lo;
     }
-    if (warp == 8) {
+    if (warp == 12) {
         if (lane == 0) {
             for (int i = 0; i < ST; ++i) {
                 mbar_init(&k_full[i], 128);
@@ -262,11 +262,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         if (ok && nt > 0) ok = mbar_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1u, DEV_ERR_ATTN_WAIT);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
-    } else if (warp < 8) {
-        // ------------------------------------------------------------------ K and V: block `w4` of each tile
-        const int w4 = warp - 4, pt = threadIdx.x - 128, key = pt >> 1, half = pt & 1, off = key & 15;
+    } else if (warp < 12) {
+        // ------------------------------------------------------------------ K (is_v 0) or V: block `w4` of each tile
+        const int is_v = (warp - 4) >> 2, w4 = warp & 3, pt = threadIdx.x & 127, key = pt >> 1, half = pt & 1, off = key & 15;
+        uint64_t* full = is_v ? v_full : k_full;
         const int32_t* table = p.block_table + (size_t)(slot_ok ? slot : 0) * p.mbps;
-        const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::BYTES;
+        const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::BYTES + (is_v ? p.v_offset : 0);
         int ids = -1;
         auto block_id = [&](int i) {  // of this warp's block of tile i; -1: none, or outside the pool
             if ((i & 31) == 0) {      // 32 tiles' ids, one per lane
@@ -282,37 +283,41 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             }
             return __shfl_sync(0xffffffffu, ids, i & 31);
         };
-        auto partial = [&](int i, int id) { return id < 0 || !is_whole(first_key((t0 + i) * 4 + w4)); };
-        auto seen_by_all = [&](int i, int id) {  // this thread's key
-            const int j = first_key((t0 + i) * 4 + w4) + off;
-            return id >= 0 && j < cmin && (j >= cmax - window || j < p.sinks);
+        uint32_t valid = 0;  // bit i % 32: tile i's block is there
+        // V of a key that some row does not see: what is not finite is set to zero and noted
+        auto hidden = [&](int i, bool in) {
+            const int j0 = first_key((t0 + i) * 4 + w4), j = j0 + off;
+            return !(in && (is_whole(j0) || (j < cmin && (j >= cmax - window || j < p.sinks))));
         };
-        // 16-byte piece c of this thread's half row of a tile's K (v = 0) or V
-        auto piece = [&](int st, int v, int c) {
-            const int ch = half * (D / 16) + c;  // of D / 8
-            return smem + L::RING + st * L::STAGE + (v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
+        auto clean = [&](uint4& u) {
+            uint32_t* o = &u.x;
+            bool bad = false;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, bad = true;
+                if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, bad = true;
+            }
+            return bad;
+        };
+        auto wait_empty = [&](int i) {  // the stage of tile i >= ST has been read
+            ok = mbar_wait(&empty[i % ST], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
+            ok = __all_sync(0xffffffffu, ok);
         };
         if constexpr (FMT == kWinQ4) {
             // codes: this warp's chunks through its own ring, RAW - 1 tiles ahead
-            const uint32_t raw = smem_u32(smem + L::CODES) + w4 * L::RAW * 2 * G::BYTES;
-            uint32_t valid = 0;  // bit i % 32: tile i's block is there
+            const uint32_t raw = smem_u32(smem + L::CODES) + (warp - 4) * L::RAW * G::BYTES;
             auto fetch = [&](int i) {
                 const int id = i < nt ? block_id(i) : -1;
                 valid = id >= 0 ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
                 if (id >= 0) {
                     const uint8_t* src = base + (uint64_t)(uint32_t)id * p.block_bytes;
-                    const uint32_t dst = raw + (i % L::RAW) * 2 * G::BYTES;
+                    const uint32_t dst = raw + (i % L::RAW) * G::BYTES;
 #pragma unroll
-                    for (int v = 0; v < 2; ++v)
-#pragma unroll
-                        for (int c = 0; c < G::BYTES / 16; c += 32)
-                            if (c + lane < G::BYTES / 16)
-                                cp_async16(dst + v * G::BYTES + (c + lane) * 16, src + v * p.v_offset + (c + lane) * 16);
+                    for (int c = 0; c < G::BYTES / 16; c += 32)
+                        if (c + lane < G::BYTES / 16) cp_async16(dst + (c + lane) * 16, src + (c + lane) * 16);
                 }
                 cp_async_commit();
             };
-#pragma unroll
-            for (int i = 0; i < L::RAW - 1; ++i) fetch(i);
             // nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as fp16 pairs, times scale plus zero
             auto values = [&](uint32_t x, __half2 scale, __half2 zero) {
                 const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
@@ -331,127 +336,95 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 return u;
             };
+            for (int i = 0; i < L::RAW - 1; ++i) fetch(i);
+            // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), of a row of D / 8 words
+            uint8_t* to = smem + L::RING + is_v * NW * L::PANEL + key * 128;
+            const uint32_t from = raw + off * (D / 2) + half * 16 * NW;
             for (int i = 0; i < nt; ++i) {
                 const int st = i % ST;
                 cp_async_wait<L::RAW - 2>();
                 __syncwarp();  // tile i's codes are there, and every lane is done with the ring's slot of tile i - 1
                 fetch(i + L::RAW - 1);
-                const int id = (valid >> (i & 31)) & 1 ? 0 : -1;
-                // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), of a row of 4 D / 32
-                uint32_t kw[NW][4] = {}, vw[NW][4] = {};
-                float2 kp[NW], vp[NW];
+                const bool in = (valid >> (i & 31)) & 1;
+                uint32_t x[NW][4] = {};
+                __half2 scale[NW], zero[NW];
 #pragma unroll
-                for (int c = 0; c < NW; ++c) kp[c] = vp[c] = make_float2(0.f, 0.f);
-                if (id >= 0) {
-                    const uint32_t at = raw + (i % L::RAW) * 2 * G::BYTES;
+                for (int c = 0; c < NW; ++c) scale[c] = zero[c] = __floats2half2_rn(0.f, 0.f);
+                if (in) {
+                    const uint32_t slot_at = (i % L::RAW) * G::BYTES;
 #pragma unroll
                     for (int c = 0; c < NW; ++c) {
-                        lds_words(kw[c], at + off * (D / 2) + half * 16 * NW + 16 * c);
-                        lds_words(vw[c], at + G::BYTES + off * (D / 2) + half * 16 * NW + 16 * c);
-                        kp[c] = lds_half2(at + Q4Layout<D>::PARAMS + c * 64 + off * 4);
-                        vp[c] = lds_half2(at + G::BYTES + Q4Layout<D>::PARAMS + c * 64 + off * 4);
+                        lds_words(x[c], from + slot_at + 16 * c);
+                        const float2 prm = lds_half2(raw + slot_at + Q4Layout<D>::PARAMS + c * 64 + off * 4);
+                        scale[c] = __float2half2_rn(prm.x);
+                        zero[c] = __float2half2_rn(prm.y);
                     }
                 }
                 if (i >= ST) {
-                    ok = mbar_wait(&empty[st], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
-                    ok = __all_sync(0xffffffffu, ok);
+                    wait_empty(i);
                     if (!ok) break;
                 }
-                if (lane == 0) s_here[st][w4] = id >= 0;
-                const bool part = partial(i, id), all = seen_by_all(i, id);
-                // word c of the half row: channels 64 w + 8 ii .. + 7, w = c % NW, ii = 4 half + c / NW
-                auto at = [&](int v, int c) {
-                    const int ii = 4 * half + c / NW;
-                    return smem + L::RING + st * L::STAGE + (v * NW + c % NW) * L::PANEL + key * 128 + ((ii ^ (key & 7)) << 4);
-                };
-#pragma unroll
-                for (int c = 0; c < 4 * NW; ++c)
-                    *reinterpret_cast<uint4*>(at(0, c)) = values(kw[c >> 2][c & 3], __float2half2_rn(kp[c % NW].x), __float2half2_rn(kp[c % NW].y));
-                fence_proxy_async_smem();
-                mbar_arrive(&k_full[st]);
+                if (!is_v && lane == 0) s_here[st][w4] = in;
+                const bool check = is_v && hidden(i, in);
                 bool bad = false;
 #pragma unroll
                 for (int c = 0; c < 4 * NW; ++c) {
-                    uint4 u = values(vw[c >> 2][c & 3], __float2half2_rn(vp[c % NW].x), __float2half2_rn(vp[c % NW].y));
-                    if (part && !all) {
-                        uint32_t* o = &u.x;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, bad = true;
-                            if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, bad = true;
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(at(1, c)) = u;
+                    uint4 u = values(x[c >> 2][c & 3], scale[c % NW], zero[c % NW]);
+                    if (check) bad |= clean(u);
+                    // channels 64 w + 8 ii .. + 7, w = c % NW
+                    const int ii = 4 * half + c / NW;
+                    *reinterpret_cast<uint4*>(to + st * L::STAGE + (c % NW) * L::PANEL + ((ii ^ (key & 7)) << 4)) = u;
                 }
-                if (part) s_bad[st][pt] = bad;
+                if (is_v) s_bad[st][pt] = bad;
                 fence_proxy_async_smem();
-                mbar_arrive(&v_full[st]);
+                mbar_arrive(&full[st]);
             }
-            cp_async_wait<0>();
         } else {
-            auto issue = [&](int i) {  // tile i's copies, K and V a group each
+            // 16-byte piece c of this thread's half row of a tile
+            auto piece = [&](int st, int c) {
+                const int ch = half * (D / 16) + c;  // of D / 8
+                return smem + L::RING + st * L::STAGE + (is_v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
+            };
+            auto fetch = [&](int i) {  // tile i's copies, a group
                 const int st = i % ST, id = i < nt ? block_id(i) : -1;
-                if (i < nt && lane == 0) s_here[st][w4] = id >= 0;
+                valid = id >= 0 ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
+                if (i < nt) {
+                    if (!is_v && lane == 0) s_here[st][w4] = id >= 0;
+                    const uint8_t* src = base + (uint64_t)(uint32_t)max(id, 0) * p.block_bytes + off * (2 * D) + half * D;
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    if (i < nt) {
-                        const uint8_t* src = base + (uint64_t)(uint32_t)max(id, 0) * p.block_bytes + (v ? p.v_offset : 0) +
-                                             off * (2 * D) + half * D;
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c) {
-                            if (id >= 0) cp_async16(smem_u32(piece(st, v, c)), src + 16 * c);
-                            else *reinterpret_cast<uint4*>(piece(st, v, c)) = make_uint4(0, 0, 0, 0);
-                        }
+                    for (int c = 0; c < D / 16; ++c) {
+                        if (id >= 0) cp_async16(smem_u32(piece(st, c)), src + 16 * c);
+                        else *reinterpret_cast<uint4*>(piece(st, c)) = make_uint4(0, 0, 0, 0);
                     }
-                    cp_async_commit();
                 }
-                return id;
+                cp_async_commit();
             };
-            uint32_t valid = 0;  // bit i % 32: tile i's block is there
-            auto start = [&](int i) {
-                const bool in = issue(i) >= 0;
-                valid = in ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
-            };
-#pragma unroll
-            for (int i = 0; i < ST - 1; ++i) start(i);
+            for (int i = 0; i < ST - 1; ++i) fetch(i);
             for (int i = 0; i < nt; ++i) {
-                const int st = i % ST, id = (valid >> (i & 31)) & 1 ? 0 : -1;
-                cp_async_wait<2 * (ST - 1) - 1>();
-                fence_proxy_async_smem();
-                mbar_arrive(&k_full[st]);
-                cp_async_wait<2 * (ST - 1) - 2>();
-                if (partial(i, id)) {
+                const int st = i % ST;
+                cp_async_wait<ST - 2>();
+                if (is_v) {
                     bool bad = false;
-                    if (!seen_by_all(i, id)) {
+                    if (hidden(i, (valid >> (i & 31)) & 1)) {
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c) {
-                            uint4 u = *reinterpret_cast<const uint4*>(piece(st, 1, c));
-                            uint32_t* o = &u.x;
-                            bool here = false;
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, here = true;
-                                if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, here = true;
-                            }
-                            if (here) *reinterpret_cast<uint4*>(piece(st, 1, c)) = u;
-                            bad |= here;
+                            uint4 u = *reinterpret_cast<const uint4*>(piece(st, c));
+                            if (clean(u)) *reinterpret_cast<uint4*>(piece(st, c)) = u, bad = true;
                         }
                     }
                     s_bad[st][pt] = bad;
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(&v_full[st]);
+                mbar_arrive(&full[st]);
                 // the next tile takes the stage of i - 1, whose products need nothing past tile i
-                const int next = i + ST - 1;
-                if (next < nt && i >= 1) {
-                    ok = mbar_wait(&empty[next % ST], (uint32_t)(next / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
-                    ok = __all_sync(0xffffffffu, ok);
+                if (i >= 1 && i + ST - 1 < nt) {
+                    wait_empty(i + ST - 1);
                     if (!ok) break;
                 }
-                start(next);
+                fetch(i + ST - 1);
             }
-            cp_async_wait<0>();
         }
+        cp_async_wait<0>();
     } else if (lane == 0) {
         // ------------------------------------------------------------------ products
         const uint32_t idesc_s = make_idesc_f16(128, 64), idesc_o = make_idesc_f16(128, D) | (1u << 16);  // V is MN-major
@@ -558,7 +531,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem, 256);
+    if (warp == 12) tmem_dealloc(tmem, 256);
     if (splits == 1) return;
     cluster_sync();
     for (int j = (int)rank * (kChunkThreads / 32) + warp; j < rows * (D / 32); j += (int)splits * (kChunkThreads / 32)) {
