@@ -24,6 +24,13 @@ namespace qtts {
 
 constexpr int kChunkThreads = 416;  // 4 softmax warps, 4 for K, 4 for V, 1 issuing warp
 
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 template <int FMT, int D>
 struct ChunkLayout {
     static constexpr int NW = D / 64;
@@ -127,10 +134,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int row = first_row + (k0 + k) * RPI;
-                float amax = max_nan(max_nan(fabsf(u[k].x), fabsf(u[k].y)), max_nan(fabsf(u[k].z), fabsf(u[k].w)));
-#pragma unroll
-                for (int x = 1; x < LPR; x <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, x));
-                const int ex = max((int)(__float_as_uint(amax) >> 23), 12);
+                // magnitudes order as integers do; NaN is above infinity
+                uint32_t top = max(max(__float_as_uint(u[k].x) & 0x7fffffffu, __float_as_uint(u[k].y) & 0x7fffffffu),
+                                   max(__float_as_uint(u[k].z) & 0x7fffffffu, __float_as_uint(u[k].w) & 0x7fffffffu));
+                top = __reduce_max_sync(RPI == 1 ? 0xffffffffu : 0xffffu << (lane & 16), top);
+                const int ex = max((int)(top >> 23), 12);
                 const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
                 uint2 h = make_uint2(pack_h2(u[k].x * up, u[k].y * up), pack_h2(u[k].z * up, u[k].w * up));
                 if constexpr (FMT == kWinQ4) {
@@ -425,19 +433,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             }
         }
         cp_async_wait<0>();
-    } else if (lane == 0) {
+    } else {
         // ------------------------------------------------------------------ products
+        // The whole warp walks the loop and one lane issues, so that descriptors stay uniform values.
+        const bool lead = elect_one();
         const uint32_t idesc_s = make_idesc_f16(128, 64), idesc_o = make_idesc_f16(128, D) | (1u << 16);  // V is MN-major
-        const uint32_t q_at = smem_u32(smem + L::Q);
+        // descriptors of the buffers' starts; a step's is an addition to the address field (16-byte units)
+        const uint64_t q_desc = make_sw128_desc(smem_u32(smem + L::Q)), k_desc = make_sw128_desc(smem_u32(smem + L::RING)),
+                       p_desc = make_sw128_desc(smem_u32(smem + L::P)),
+                       v_desc = make_sw128_mn_desc(smem_u32(smem + L::RING + NW * L::PANEL), L::PANEL);
         auto issue_s = [&](int i) {
             if (!mbar_wait(&k_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT)) return false;
             tc_fence_after();
-            const uint32_t k_at = smem_u32(smem + L::RING + (i % ST) * L::STAGE);
+            const uint64_t kd = k_desc + (uint32_t)((i % ST) * (L::STAGE >> 4));
+            const uint32_t d = tmem + (i & 1) * 64;
+            if (lead) {
 #pragma unroll
-            for (int kk = 0; kk < 4 * NW; ++kk)
-                umma_bf16(tmem + (i & 1) * 64, make_sw128_desc(q_at + (kk >> 2) * 16384) + 2 * (kk & 3),
-                          make_sw128_desc(k_at + (kk >> 2) * L::PANEL) + 2 * (kk & 3), idesc_s, kk ? 1u : 0u);
-            umma_commit(&s_full[i & 1]);
+                for (int kk = 0; kk < 4 * NW; ++kk)
+                    umma_bf16(d, q_desc + ((kk >> 2) * (16384 >> 4) + 2 * (kk & 3)),
+                              kd + ((kk >> 2) * (L::PANEL >> 4) + 2 * (kk & 3)), idesc_s, kk ? 1u : 0u);
+                umma_commit(&s_full[i & 1]);
+            }
             return true;
         };
         if (nt > 0) ok = issue_s(0);
@@ -445,18 +461,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             if (i + 1 < nt) ok = issue_s(i + 1);
             ok = ok && mbar_wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u, DEV_ERR_ATTN_WAIT);
             ok = ok && mbar_wait(&v_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t p_at = smem_u32(smem + L::P + (i & 1) * 16384);
-            const uint32_t v_at = smem_u32(smem + L::RING + (i % ST) * L::STAGE + NW * L::PANEL);
+            const uint64_t pd = p_desc + (uint32_t)((i & 1) * (16384 >> 4)), vd = v_desc + (uint32_t)((i % ST) * (L::STAGE >> 4));
+            if (lead) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                umma_bf16(tmem + 128u, make_sw128_desc(p_at) + 2 * kk, make_sw128_mn_desc(v_at + kk * 2048, L::PANEL), idesc_o,
-                          (i > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&empty[i % ST]);
-            umma_commit(&pv_done[i & 1]);
+                for (int kk = 0; kk < 4; ++kk)
+                    umma_bf16(tmem + 128u, pd + 2 * kk, vd + kk * (2048 >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                umma_commit(&empty[i % ST]);
+                umma_commit(&pv_done[i & 1]);
+            }
+            __syncwarp();
         }
-        if (!ok) {  // every product issued so far ends before TMEM is given back
+        if (!__all_sync(0xffffffffu, ok) && lead) {  // every product issued so far ends before TMEM is given back
             __shared__ uint64_t drain;
             mbar_init(&drain, 1);
             fence_mbar_init();
