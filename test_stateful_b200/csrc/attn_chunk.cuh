@@ -24,6 +24,26 @@ namespace qtts {
 
 constexpr int kChunkThreads = 416;  // 4 softmax warps, 4 for K, 4 for V, 1 issuing warp
 
+// 32 lanes x 32 bits, 64 consecutive columns, both loads under way before the wait
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+    uint32_t r[64];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t* q = r + 32 * h;
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+              "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]),
+              "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]),
+              "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+            : "r"(taddr + 32 * h));
+    }
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -44,7 +64,9 @@ struct ChunkLayout {
     static constexpr int CODES = P + 2 * 128 * 128;   // [K, V][warp][RAW] chunks
     static constexpr int SMEM = CODES + 4 * RAW * 2 * WinChunk<FMT, D>::BYTES + 1024;
     static constexpr int PART = D + 4;                // floats per row of a partial output (no bank met twice)
-    static_assert(128 * PART * 4 <= ST * STAGE + 2 * 128 * 128, "a partial output replaces ring and P");
+    static constexpr int ROWB = 2 * D + 16;           // bytes per row of a bf16 output
+    static_assert(128 * PART * 4 <= ST * STAGE + 2 * 128 * 128 && 2 * 128 * ROWB <= ST * STAGE + 2 * 128 * 128,
+                  "outputs replace ring and P");
     static_assert(SMEM + 4096 <= 227 * 1024, "tile exceeds shared memory");
 };
 
@@ -55,11 +77,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     constexpr int NW = L::NW, ST = L::ST;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t k_full[ST], v_full[ST], empty[ST], s_full[2], p_full[2], pv_done[2];
+    __shared__ uint64_t k_full[ST], v_full[ST], empty[ST], s_full[2], p_full[2], pv_done[2], q_full;
     __shared__ uint32_t s_tmem;
     __shared__ int s_lim[4][2];                                 // contexts' extremes per softmax warp
     __shared__ __align__(16) uint8_t s_bad[ST][128];            // per key and half: V had a value that is not finite
-    __shared__ uint8_t s_here[ST][4];                           // per block: it is there and in the pool
+    __shared__ __align__(4) uint8_t s_here[ST][4];              // per block: it is there and in the pool
+    __shared__ __align__(4) uint8_t s_some_bad[ST][4];          // per block: some key is bad
     __shared__ float s_part[128][2];                            // (max, sum) per row
     __shared__ float s_sf[128];                                 // accumulator -> log2 units, per row
 
@@ -107,27 +130,59 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 mbar_init(&p_full[i], 128);
                 mbar_init(&pv_done[i], 1);
             }
+            mbar_init(&q_full, 128);
             fence_mbar_init();
         }
         __syncwarp();
         tmem_alloc(&s_tmem, 256);
         tmem_relinquish();
     }
-    // Q: warps 0-7 take 16 rows each, a row (D = 64: two) at a time, four channels a lane, the next
-    // four steps' loads under way
-    if (warp < 8) {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    int cmax = 0, cmin = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cmax = max(cmax, s_lim[i][0]), cmin = min(cmin, s_lim[i][1]);
+    const int nb_end = (cmax + 15) >> 4;
+    const int nb_sink = min((min(p.sinks, cmax) + 15) >> 4, nb_end);
+    const int first = max(nb_sink, cmax > 0 ? max(0, cmin - window) >> 4 : 0);
+    const int past_sinks = first - nb_sink;
+    const int nb = nb_sink + max(0, nb_end - first);
+    const int all_tiles = (nb + 3) >> 2;
+    const int even = all_tiles / (int)splits, rest = all_tiles % (int)splits;
+    const int t0 = (int)rank * even + min((int)rank, rest), nt = even + ((int)rank < rest);  // this CTA's tiles
+    auto first_key = [&](int pos) { return (pos < nb_sink ? pos : pos + past_sinks) * 16; };
+    auto is_whole = [&](int j0) { return j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks); };
+
+    // tiles [whole0, whole1) of all hold only blocks that every row sees whole (if they are in the pool)
+    const int below_all = cmin >> 4;  // blocks that end at or before every row's context
+    int whole0 = 0, whole1 = min(nb, below_all >= first ? nb_sink + below_all - first : min(nb_sink, below_all)) >> 2;
+    if (cmax > window) {  // blocks from the latest window's start on, or all within the sinks
+        const int from = nb_sink + max(0, ((cmax - window + 15) >> 4) - first);
+        whole0 = (from + 3) >> 2;
+        if (from <= nb_sink && (nb_sink == 0 || nb_sink * 16 <= p.sinks)) whole0 = 0;
+    }
+
+    bool ok = true;  // a wait that ran out ends the thread's loop
+    float m = -INFINITY, mu = 0.f, l = 0.f;
+    if (warp < 4) {
+        // ------------------------------------------------------------------ Q, then softmax
+        // Q: a warp takes 32 rows, one (D = 64: two) at a time, four channels a lane, the next four
+        // steps' loads under way
         constexpr int RPI = 128 / D, LPR = 32 / RPI;  // rows per step, lanes per row
-        const int c = lane % LPR, first_row = warp * 16 + lane / LPR;
+        const int c = lane % LPR, first_row = warp * 32 + lane / LPR;
         auto fetch = [&](int k) {
             const int row = first_row + k * RPI;
-            return row < rows && k * RPI < 16 ? __ldg(reinterpret_cast<const float4*>(p.q + head_row(row) * D) + c)
+            return row < rows && k * RPI < 32 ? __ldg(reinterpret_cast<const float4*>(p.q + head_row(row) * D) + c)
                                               : make_float4(0.f, 0.f, 0.f, 0.f);
         };
         float4 u[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) u[k] = fetch(k);
 #pragma unroll 1
-        for (int k0 = 0; k0 < 16 / RPI; k0 += 4) {
+        for (int k0 = 0; k0 < 32 / RPI; k0 += 4) {
             float4 next[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) next[k] = fetch(k0 + 4 + k);
@@ -153,32 +208,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 u[k] = next[k];
             }
         }
-    }
-    fence_proxy_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = s_tmem;
-
-    int cmax = 0, cmin = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) cmax = max(cmax, s_lim[i][0]), cmin = min(cmin, s_lim[i][1]);
-    const int nb_end = (cmax + 15) >> 4;
-    const int nb_sink = min((min(p.sinks, cmax) + 15) >> 4, nb_end);
-    const int first = max(nb_sink, cmax > 0 ? max(0, cmin - window) >> 4 : 0);
-    const int past_sinks = first - nb_sink;
-    const int nb = nb_sink + max(0, nb_end - first);
-    const int all_tiles = (nb + 3) >> 2;
-    const int even = all_tiles / (int)splits, rest = all_tiles % (int)splits;
-    const int t0 = (int)rank * even + min((int)rank, rest), nt = even + ((int)rank < rest);  // this CTA's tiles
-    auto first_key = [&](int pos) { return (pos < nb_sink ? pos : pos + past_sinks) * 16; };
-    auto is_whole = [&](int j0) { return j0 + 16 <= cmin && (j0 >= cmax - window || j0 + 16 <= p.sinks); };
-
-    bool ok = true;  // a wait that ran out ends the thread's loop
-    const float sf = s_sf[r & 127];
-    float m = -INFINITY, mu = 0.f, l = 0.f;
-    if (warp < 4) {
-        // ------------------------------------------------------------------ softmax
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full);
+        __syncwarp();  // the warp's rows are its own lanes'
+        const float sf = s_sf[r];
         const uint32_t lanes = tmem + ((uint32_t)warp << 21);
         for (int i = 0; i < nt && ok; ++i) {
             const int st = i % ST, pos = (t0 + i) * 4;
@@ -188,12 +221,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             if (!ok) break;
             tc_fence_after();
             float v[64];
-            tmem_ld32(lanes + (i & 1) * 64, reinterpret_cast<float(&)[32]>(v[0]));
-            tmem_ld32(lanes + (i & 1) * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+            tmem_ld64(lanes + (i & 1) * 64, v);
             const uint32_t here = *reinterpret_cast<const uint32_t*>(s_here[st]);
-            bool whole = here == 0x01010101u;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) whole = whole && is_whole(first_key(pos + b));
+            const bool whole = here == 0x01010101u && t0 + i >= whole0 && t0 + i < whole1;
             if (!whole) {
                 ok = mbar_wait(&v_full[st], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);  // (for s_bad)
                 ok = __all_sync(0xffffffffu, ok);
@@ -207,9 +237,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     auto below = [&](int j) { return (1u << min(max(j - j0, 0), 16)) - 1u; };
                     uint32_t sees = below(ctx) & (~below(max(ctx - window, 0)) | below(p.sinks));
                     if (!there) sees = 0;
-                    const uint4 bad0 = *reinterpret_cast<const uint4*>(s_bad[st] + 32 * b);
-                    const uint4 bad1 = *reinterpret_cast<const uint4*>(s_bad[st] + 32 * b + 16);
-                    if ((bad0.x | bad0.y | bad0.z | bad0.w | bad1.x | bad1.y | bad1.z | bad1.w) != 0) {
+                    if (s_some_bad[st][b]) {
                         for (int k = 0; k < 16; ++k)  // its V was taken out: the row becomes NaN
                             if (((sees >> k) & 1) && *reinterpret_cast<const uint16_t*>(s_bad[st] + 32 * b + 2 * k))
                                 l = __int_as_float(0x7fffffff);
@@ -383,7 +411,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     const int ii = 4 * half + c / NW;
                     *reinterpret_cast<uint4*>(to + st * L::STAGE + (c % NW) * L::PANEL + ((ii ^ (key & 7)) << 4)) = u;
                 }
-                if (is_v) s_bad[st][pt] = bad;
+                if (is_v) {
+                    s_bad[st][pt] = bad;
+                    const bool any = __any_sync(0xffffffffu, bad);
+                    if (lane == 0) s_some_bad[st][w4] = any;
+                }
                 fence_proxy_async_smem();
                 mbar_arrive(&full[st]);
             }
@@ -421,6 +453,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                         }
                     }
                     s_bad[st][pt] = bad;
+                    const bool any = __any_sync(0xffffffffu, bad);
+                    if (lane == 0) s_some_bad[st][w4] = any;
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(&full[st]);
@@ -456,7 +490,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             }
             return true;
         };
-        if (nt > 0) ok = issue_s(0);
+        if (nt > 0) ok = mbar_wait(&q_full, 0, DEV_ERR_ATTN_WAIT) && issue_s(0);
         for (int i = 0; i < nt && ok; ++i) {
             if (i + 1 < nt) ok = issue_s(i + 1);
             ok = ok && mbar_wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u, DEV_ERR_ATTN_WAIT);
@@ -491,66 +525,60 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     if (warp < 4) {
         const uint32_t lanes = tmem + ((uint32_t)warp << 21) + 128;
         const bool sum = ok && nt > 0 && l != 0.f;  // else zeros (NaN counts as a sum)
-        const float inv = sum ? 1.f / l : 0.f;
+        const float inv = splits == 1 ? 1.f / l : 1.f;
+        uint8_t* staged = smem + L::RING;  // [row][ROWB] bf16, then the low halves
         s_part[r][0] = m;
         s_part[r][1] = ok ? l : 0.f;
-        constexpr int ROWB = 2 * D + 16;  // bytes of a staged output row
-        uint8_t* rows_at = smem + L::RING + warp * 64 * ROWB;
-        static_assert(4 * 64 * ROWB <= ST * L::STAGE, "staged output rows replace the ring");
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-            float x[16], y[16];
-            tmem_ld16(lanes + c, x);
+        for (int c = 0; c < D; c += 32) {
+            float x[32], y[32];
+            tmem_ld32(lanes + c, x);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
+            for (int k = 0; k < 32; ++k) {
                 // 4 bits: position 8 n + k of V holds channel 8 n + k / 2 + 4 (k % 2)
-                const int ch = FMT == kWinQ4 ? (k & 8) + ((k & 7) >> 1) + 4 * (k & 1) : k;
-                y[ch] = sum ? (splits == 1 ? x[k] * inv : x[k]) : 0.f;
+                const int ch = FMT == kWinQ4 ? (k & 24) + ((k & 7) >> 1) + 4 * (k & 1) : k;
+                y[ch] = sum ? x[k] * inv : 0.f;
             }
             if (splits > 1) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < 8; ++k)
                     *reinterpret_cast<float4*>(part + r * L::PART + c + 4 * k) =
                         make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
             } else {
-                uint32_t hi[8], lo[8];
+                uint8_t* at = staged + r * L::ROWB + 2 * c;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * k], y[2 * k + 1]);
-                    const float2 f = __bfloat1622float2(h);
-                    const __nv_bfloat162 g = __floats2bfloat162_rn(y[2 * k] - f.x, y[2 * k + 1] - f.y);
-                    hi[k] = *reinterpret_cast<const uint32_t*>(&h);
-                    lo[k] = *reinterpret_cast<const uint32_t*>(&g);
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t hi[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) hi[j] = pack_bf2(y[8 * k + 2 * j], y[8 * k + 2 * j + 1]);
+                    *reinterpret_cast<uint4*>(at + 16 * k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (p.out_lo) {
+                        uint32_t lo[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            lo[j] = pack_bf2(y[8 * k + 2 * j] - __uint_as_float(hi[j] << 16),
+                                             y[8 * k + 2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
+                        *reinterpret_cast<uint4*>(at + 128 * L::ROWB + 16 * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
                 }
-                uint4* o = reinterpret_cast<uint4*>(rows_at + lane * ROWB + 2 * c);
-                o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                if (p.out_lo) {
-                    uint4* ol = reinterpret_cast<uint4*>(rows_at + 32 * ROWB + lane * ROWB + 2 * c);
-                    ol[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    ol[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-                }
-            }
-        }
-        if (splits == 1) {
-            // a warp's 32 rows leave through shared memory, so that its stores are whole rows
-            __syncwarp();
-#pragma unroll 4
-            for (int k = lane; k < 32 * (D / 8); k += 32) {
-                const int row = k / (D / 8), c = k % (D / 8);
-                if (warp * 32 + row >= rows) break;
-                const size_t at = out_at(warp * 32 + row, 8 * c);
-                *reinterpret_cast<uint4*>(p.out + at) = *reinterpret_cast<const uint4*>(rows_at + row * ROWB + 16 * c);
-                if (p.out_lo)
-                    *reinterpret_cast<uint4*>(p.out_lo + at) =
-                        *reinterpret_cast<const uint4*>(rows_at + 32 * ROWB + row * ROWB + 16 * c);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 12) tmem_dealloc(tmem, 256);
-    if (splits == 1) return;
+    if (splits == 1) {
+        // whole rows leave shared memory
+        for (int k = threadIdx.x; k < rows * (D / 8); k += kChunkThreads) {
+            const int row = k / (D / 8), c = k % (D / 8);
+            const size_t at = out_at(row, 8 * c);
+            const uint8_t* from = smem + L::RING + row * L::ROWB + 16 * c;
+            *reinterpret_cast<uint4*>(p.out + at) = *reinterpret_cast<const uint4*>(from);
+            if (p.out_lo)
+                *reinterpret_cast<uint4*>(p.out_lo + at) = *reinterpret_cast<const uint4*>(from + 128 * L::ROWB);
+        }
+        return;
+    }
     cluster_sync();
     for (int j = (int)rank * (kChunkThreads / 32) + warp; j < rows * (D / 32); j += (int)splits * (kChunkThreads / 32)) {
         const int row = j / (D / 32), d = (j % (D / 32)) * 32 + lane;

@@ -116,6 +116,10 @@ __device__ __forceinline__ float2 lds_half2(uint32_t addr) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(addr));
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
+__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
 // A chunk in shared memory, 16-byte pieces permuted so that the fragment reads meet no bank twice.
