@@ -100,6 +100,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     const int row0 = stream * p.S + q0;
     const size_t head0 = (size_t)row0 * p.num_heads + kvh * p.group;  // q and out row (head) of tile row 0
     auto head_row = [&](int row) { return head0 + (uint32_t)(p.by_group.div(row) * (p.num_heads - p.group) + row); };
+    // Q, on its way while the contexts are read: warps 0-11 take every twelfth row (D = 64: pair of rows),
+    // four channels a lane
+    constexpr int RPI = 128 / D, LPR = 32 / RPI;  // rows per step, lanes per row
+    auto q_row = [&](int k) { return (warp + 12 * k) * RPI + lane / LPR; };
+    float4 q_now[6], q_next[6];
+#pragma unroll
+    for (int k = 0; k < 12; ++k) {
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (warp < 12 && q_row(k) < rows) u = __ldg(reinterpret_cast<const float4*>(p.q + head_row(q_row(k)) * D) + lane % LPR);
+        if (k < 6) q_now[k] = u;
+        else q_next[k - 6] = u;
+    }
     const int limit = min(p.max_ctx, p.mbps * 16);
     const int window = p.window > 0 ? p.window : 0x7fffffff;
     const int slot = __ldg(p.row_slot + row0);
@@ -130,7 +142,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 mbar_init(&p_full[i], 128);
                 mbar_init(&pv_done[i], 1);
             }
-            mbar_init(&q_full, 128);
+            mbar_init(&q_full, 384);
             fence_mbar_init();
         }
         __syncwarp();
@@ -166,36 +178,96 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     }
 
     bool ok = true;  // a wait that ran out ends the thread's loop
-    float m = -INFINITY, mu = 0.f, l = 0.f;
-    if (warp < 4) {
-        // ------------------------------------------------------------------ Q, then softmax
-        // Q: a warp takes 32 rows, one (D = 64: two) at a time, four channels a lane, the next four
-        // steps' loads under way
-        constexpr int RPI = 128 / D, LPR = 32 / RPI;  // rows per step, lanes per row
-        const int c = lane % LPR, first_row = warp * 32 + lane / LPR;
-        auto fetch = [&](int k) {
-            const int row = first_row + k * RPI;
-            return row < rows && k * RPI < 32 ? __ldg(reinterpret_cast<const float4*>(p.q + head_row(row) * D) + c)
-                                              : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        float4 u[4];
+    // ---------------------------------------------------------------------- loading warps: where they are
+    const int is_v = (warp - 4) >> 2, w4 = warp & 3, pt = threadIdx.x & 127, key = pt >> 1, half = pt & 1, off = key & 15;
+    uint64_t* full = is_v ? v_full : k_full;
+    const int32_t* table = p.block_table + (size_t)(slot_ok ? slot : 0) * p.mbps;
+    const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::BYTES + (is_v ? p.v_offset : 0);
+    int ids = -1;
+    auto block_id = [&](int i) {  // of this warp's block of tile i; -1: none, or outside the pool
+        if ((i & 31) == 0) {      // 32 tiles' ids, one per lane
+            const int pos = (t0 + i + lane) * 4 + w4;
+            ids = -1;
+            if (i + lane < nt && pos < nb) {
+                ids = __ldg(table + (first_key(pos) >> 4));
+                if (ids < 0 || ids >= p.num_blocks) {
+                    record_error(DEV_ERR_ATTN_BOUNDS);
+                    ids = -1;
+                }
+            }
+        }
+        return __shfl_sync(0xffffffffu, ids, i & 31);
+    };
+    uint32_t valid = 0;  // bit i % 32: tile i's block is there
+    // V of a key that some row does not see: what is not finite is set to zero and noted
+    auto hidden = [&](int i, bool in) {
+        const int j0 = first_key((t0 + i) * 4 + w4), j = j0 + off;
+        return !(in && (is_whole(j0) || (j < cmin && (j >= cmax - window || j < p.sinks))));
+    };
+    auto clean = [&](uint4& u) {
+        uint32_t* o = &u.x;
+        bool bad = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = fetch(k);
+        for (int x = 0; x < 4; ++x) {
+            if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, bad = true;
+            if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, bad = true;
+        }
+        return bad;
+    };
+    auto wait_empty = [&](int i) {  // the stage of tile i >= ST has been read
+        ok = mbar_wait(&empty[i % ST], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
+        ok = __all_sync(0xffffffffu, ok);
+    };
+    // 4 bits: codes through the warp's own ring, RAW - 1 tiles ahead
+    const uint32_t raw = smem_u32(smem + L::CODES) + (warp - 4) * L::RAW * G::BYTES;
+    // fp16: 16-byte piece c of this thread's half row of a tile
+    auto piece = [&](int st, int c) {
+        const int ch = half * (D / 16) + c;  // of D / 8
+        return smem + L::RING + st * L::STAGE + (is_v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
+    };
+    auto fetch = [&](int i) {  // tile i's copies, a group
+        const int id = i < nt ? block_id(i) : -1;
+        valid = id >= 0 ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
+        const uint8_t* src = base + (uint64_t)(uint32_t)max(id, 0) * p.block_bytes;
+        if constexpr (FMT == kWinQ4) {
+            if (id >= 0) {
+                const uint32_t dst = raw + (i % L::RAW) * G::BYTES;
+#pragma unroll
+                for (int c = 0; c < G::BYTES / 16; c += 32)
+                    if (c + lane < G::BYTES / 16) cp_async16(dst + (c + lane) * 16, src + (c + lane) * 16);
+            }
+        } else if (i < nt) {
+            const int st = i % ST;
+            if (!is_v && lane == 0) s_here[st][w4] = id >= 0;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                if (id >= 0) cp_async16(smem_u32(piece(st, c)), src + off * (2 * D) + half * D + 16 * c);
+                else *reinterpret_cast<uint4*>(piece(st, c)) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        cp_async_commit();
+    };
+    constexpr int AHEAD = FMT == kWinQ4 ? L::RAW - 1 : ST - 1;
+    if (warp >= 4 && warp < 12)
+        for (int i = 0; i < AHEAD; ++i) fetch(i);
+
+    // ---------------------------------------------------------------------- Q to shared memory
+    if (warp < 12) {
+        const int c = lane % LPR;
 #pragma unroll 1
-        for (int k0 = 0; k0 < 32 / RPI; k0 += 4) {
-            float4 next[4];
+        for (int k0 = 0; k0 < 12; k0 += 6) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) next[k] = fetch(k0 + 4 + k);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int row = first_row + (k0 + k) * RPI;
+            for (int k = 0; k < 6; ++k) {
+                const int row = q_row(k0 + k);
+                if (row >= 128) break;
+                const float4 u = q_now[k];
                 // magnitudes order as integers do; NaN is above infinity
-                uint32_t top = max(max(__float_as_uint(u[k].x) & 0x7fffffffu, __float_as_uint(u[k].y) & 0x7fffffffu),
-                                   max(__float_as_uint(u[k].z) & 0x7fffffffu, __float_as_uint(u[k].w) & 0x7fffffffu));
+                uint32_t top = max(max(__float_as_uint(u.x) & 0x7fffffffu, __float_as_uint(u.y) & 0x7fffffffu),
+                                   max(__float_as_uint(u.z) & 0x7fffffffu, __float_as_uint(u.w) & 0x7fffffffu));
                 top = __reduce_max_sync(RPI == 1 ? 0xffffffffu : 0xffffu << (lane & 16), top);
                 const int ex = max((int)(top >> 23), 12);
                 const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
-                uint2 h = make_uint2(pack_h2(u[k].x * up, u[k].y * up), pack_h2(u[k].z * up, u[k].w * up));
+                uint2 h = make_uint2(pack_h2(u.x * up, u.y * up), pack_h2(u.z * up, u.w * up));
                 if constexpr (FMT == kWinQ4) {
                     // the channel order in which nibbles come apart (below): 0 4 1 5 2 6 3 7 of each eight.
                     // An even lane holds 0 1 2 3 and makes 0 4 1 5, the odd one beside it 4 5 6 7 and 2 6 3 7
@@ -205,12 +277,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 *reinterpret_cast<uint2*>(smem + L::Q + (c >> 4) * 16384 + sw128_off(row, (c & 15) * 4)) = h;
                 if (c == 0) s_sf[row] = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
-                u[k] = next[k];
             }
+#pragma unroll
+            for (int k = 0; k < 6; ++k) q_now[k] = q_next[k];
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_full);
-        __syncwarp();  // the warp's rows are its own lanes'
+    }
+
+    float m = -INFINITY, mu = 0.f, l = 0.f;
+    if (warp < 4) {
+        // ------------------------------------------------------------------ softmax
+        ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0, DEV_ERR_ATTN_WAIT));  // (for s_sf)
         const float sf = s_sf[r];
         const uint32_t lanes = tmem + ((uint32_t)warp << 21);
         for (int i = 0; i < nt && ok; ++i) {
@@ -300,60 +378,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         tc_fence_after();
     } else if (warp < 12) {
         // ------------------------------------------------------------------ K (is_v 0) or V: block `w4` of each tile
-        const int is_v = (warp - 4) >> 2, w4 = warp & 3, pt = threadIdx.x & 127, key = pt >> 1, half = pt & 1, off = key & 15;
-        uint64_t* full = is_v ? v_full : k_full;
-        const int32_t* table = p.block_table + (size_t)(slot_ok ? slot : 0) * p.mbps;
-        const uint8_t* base = p.kv + ((size_t)p.layer * 2 * p.kv_heads + kvh) * G::BYTES + (is_v ? p.v_offset : 0);
-        int ids = -1;
-        auto block_id = [&](int i) {  // of this warp's block of tile i; -1: none, or outside the pool
-            if ((i & 31) == 0) {      // 32 tiles' ids, one per lane
-                const int pos = (t0 + i + lane) * 4 + w4;
-                ids = -1;
-                if (i + lane < nt && pos < nb) {
-                    ids = __ldg(table + (first_key(pos) >> 4));
-                    if (ids < 0 || ids >= p.num_blocks) {
-                        record_error(DEV_ERR_ATTN_BOUNDS);
-                        ids = -1;
-                    }
-                }
-            }
-            return __shfl_sync(0xffffffffu, ids, i & 31);
-        };
-        uint32_t valid = 0;  // bit i % 32: tile i's block is there
-        // V of a key that some row does not see: what is not finite is set to zero and noted
-        auto hidden = [&](int i, bool in) {
-            const int j0 = first_key((t0 + i) * 4 + w4), j = j0 + off;
-            return !(in && (is_whole(j0) || (j < cmin && (j >= cmax - window || j < p.sinks))));
-        };
-        auto clean = [&](uint4& u) {
-            uint32_t* o = &u.x;
-            bool bad = false;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                if ((o[x] & 0x7c00u) == 0x7c00u) o[x] &= 0xffff0000u, bad = true;
-                if ((o[x] & 0x7c000000u) == 0x7c000000u) o[x] &= 0x0000ffffu, bad = true;
-            }
-            return bad;
-        };
-        auto wait_empty = [&](int i) {  // the stage of tile i >= ST has been read
-            ok = mbar_wait(&empty[i % ST], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
-            ok = __all_sync(0xffffffffu, ok);
-        };
         if constexpr (FMT == kWinQ4) {
-            // codes: this warp's chunks through its own ring, RAW - 1 tiles ahead
-            const uint32_t raw = smem_u32(smem + L::CODES) + (warp - 4) * L::RAW * G::BYTES;
-            auto fetch = [&](int i) {
-                const int id = i < nt ? block_id(i) : -1;
-                valid = id >= 0 ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
-                if (id >= 0) {
-                    const uint8_t* src = base + (uint64_t)(uint32_t)id * p.block_bytes;
-                    const uint32_t dst = raw + (i % L::RAW) * G::BYTES;
-#pragma unroll
-                    for (int c = 0; c < G::BYTES / 16; c += 32)
-                        if (c + lane < G::BYTES / 16) cp_async16(dst + (c + lane) * 16, src + (c + lane) * 16);
-                }
-                cp_async_commit();
-            };
             // nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as fp16 pairs, times scale plus zero
             auto values = [&](uint32_t x, __half2 scale, __half2 zero) {
                 const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
@@ -372,7 +397,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 return u;
             };
-            for (int i = 0; i < L::RAW - 1; ++i) fetch(i);
             // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), of a row of D / 8 words
             uint8_t* to = smem + L::RING + is_v * NW * L::PANEL + key * 128;
             const uint32_t from = raw + off * (D / 2) + half * 16 * NW;
@@ -402,14 +426,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 }
                 if (!is_v && lane == 0) s_here[st][w4] = in;
                 const bool check = is_v && hidden(i, in);
-                bool bad = false;
+                uint4 u[4 * NW];
 #pragma unroll
-                for (int c = 0; c < 4 * NW; ++c) {
-                    uint4 u = values(x[c >> 2][c & 3], scale[c % NW], zero[c % NW]);
-                    if (check) bad |= clean(u);
-                    // channels 64 w + 8 ii .. + 7, w = c % NW
+                for (int c = 0; c < 4 * NW; ++c) u[c] = values(x[c >> 2][c & 3], scale[c % NW], zero[c % NW]);
+                bool bad = false;
+                if (check) {
+#pragma unroll
+                    for (int c = 0; c < 4 * NW; ++c) bad |= clean(u[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4 * NW; ++c) {  // channels 64 w + 8 ii .. + 7, w = c % NW
                     const int ii = 4 * half + c / NW;
-                    *reinterpret_cast<uint4*>(to + st * L::STAGE + (c % NW) * L::PANEL + ((ii ^ (key & 7)) << 4)) = u;
+                    *reinterpret_cast<uint4*>(to + st * L::STAGE + (c % NW) * L::PANEL + ((ii ^ (key & 7)) << 4)) = u[c];
                 }
                 if (is_v) {
                     s_bad[st][pt] = bad;
@@ -420,26 +448,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 mbar_arrive(&full[st]);
             }
         } else {
-            // 16-byte piece c of this thread's half row of a tile
-            auto piece = [&](int st, int c) {
-                const int ch = half * (D / 16) + c;  // of D / 8
-                return smem + L::RING + st * L::STAGE + (is_v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
-            };
-            auto fetch = [&](int i) {  // tile i's copies, a group
-                const int st = i % ST, id = i < nt ? block_id(i) : -1;
-                valid = id >= 0 ? valid | (1u << (i & 31)) : valid & ~(1u << (i & 31));
-                if (i < nt) {
-                    if (!is_v && lane == 0) s_here[st][w4] = id >= 0;
-                    const uint8_t* src = base + (uint64_t)(uint32_t)max(id, 0) * p.block_bytes + off * (2 * D) + half * D;
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        if (id >= 0) cp_async16(smem_u32(piece(st, c)), src + 16 * c);
-                        else *reinterpret_cast<uint4*>(piece(st, c)) = make_uint4(0, 0, 0, 0);
-                    }
-                }
-                cp_async_commit();
-            };
-            for (int i = 0; i < ST - 1; ++i) fetch(i);
             for (int i = 0; i < nt; ++i) {
                 const int st = i % ST;
                 cp_async_wait<ST - 2>();
