@@ -588,39 +588,76 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         return;
     }
     cluster_sync();
-    for (int j = (int)rank * (kChunkThreads / 32) + warp; j < rows * (D / 32); j += (int)splits * (kChunkThreads / 32)) {
-        const int row = j / (D / 32), d = (j % (D / 32)) * 32 + lane;
-        float mc = -INFINITY, lc = 0.f;
-        if (lane < (int)splits) {
-            mc = ld_dsmem_now(map_to_rank(smem_u32(&s_part[row][0]), lane));
-            lc = ld_dsmem_now(map_to_rank(smem_u32(&s_part[row][1]), lane));
-        }
-        float v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-            if (c < (int)splits) v[c] = ld_dsmem_now(map_to_rank(smem_u32(part + row * L::PART + d), c));
-        const float mx = warp_max(mc);
-        const float f = mc == -INFINITY ? 0.f : ex2_approx(mc - mx);
-        const float sum = warp_sum(mc == -INFINITY && lc != 0.f ? lc : lc * f);
-        float acc = 0.f;
+    // four channels a lane, a row (D = 64: two) a warp; every CTA's part is fetched at once
+    for (int j = (int)rank * (kChunkThreads / 32) + warp; j * RPI < rows; j += (int)splits * (kChunkThreads / 32)) {
+        const int row = min(j * RPI + lane / LPR, rows - 1), d = (lane % LPR) * 4;
+        const uint32_t at_o = smem_u32(part + row * L::PART + d), at_m = smem_u32(&s_part[row][0]);
+        float4 v[8];
+        float mc[8], lc[8], mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            const float fc = __shfl_sync(0xffffffffu, f, c);
-            if (c < (int)splits && fc != 0.f) acc = fmaf(v[c], fc, acc);
+            mc[c] = -INFINITY;
+            lc[c] = 0.f;
+            if (c < (int)splits) {
+                mc[c] = ld_dsmem_now(map_to_rank(at_m, c));
+                lc[c] = ld_dsmem_now(map_to_rank(at_m + 4, c));
+                v[c] = ld_dsmem_f32x4(map_to_rank(at_o, c));
+            }
         }
-        const float x = sum == 0.f ? 0.f : acc / sum;
-        const __nv_bfloat16 hi = __float2bfloat16_rn(x);
-        p.out[out_at(row, d)] = hi;
-        if (p.out_lo) p.out_lo[out_at(row, d)] = __float2bfloat16_rn(x - __bfloat162float(hi));
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mx = fmaxf(mx, mc[c]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            // a CTA without keys holds nothing, one of nothing but NaN scores a sum that is not zero
+            if (mc[c] == -INFINITY) {
+                sum += lc[c];
+            } else {
+                const float f = ex2_approx(mc[c] - mx);
+                sum = fmaf(lc[c], f, sum);
+                acc.x = fmaf(v[c].x, f, acc.x), acc.y = fmaf(v[c].y, f, acc.y);
+                acc.z = fmaf(v[c].z, f, acc.z), acc.w = fmaf(v[c].w, f, acc.w);
+            }
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float x = acc.x * inv, y = acc.y * inv, z = acc.z * inv, w = acc.w * inv;
+        const uint2 hi = make_uint2(pack_bf2(x, y), pack_bf2(z, w));
+        *reinterpret_cast<uint2*>(p.out + out_at(row, d)) = hi;
+        if (p.out_lo)
+            *reinterpret_cast<uint2*>(p.out_lo + out_at(row, d)) =
+                make_uint2(pack_bf2(x - __uint_as_float(hi.x << 16), y - __uint_as_float(hi.x & 0xffff0000u)),
+                           pack_bf2(z - __uint_as_float(hi.y << 16), w - __uint_as_float(hi.y & 0xffff0000u)));
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// Whether rows go through 128-row tiles.
+// Whether rows go through 128-row tiles (QTTS_WINDOW_TILES=0 / 1 forces it where either form can run).
+// A tile CTA costs some 7 us before its first products and after its last, the row kernel 8 rows' reading
+// of every block; tiles win once they are at least half full and the row kernel has more than a few
+// thousand (8-row tile, block) pairs or more than a wave of tiles.  Measured (us, 16 heads over 8,
+// streams x rows + past, tiles / rows, B200):
+//   4 bits  1 x 64 + 500   13.3 / 8.9     1 x 128 + 500  13.5 / 12.7   1 x 256 + 500  15.0 / 22.2
+//           8 x 16 + 500   14.1 / 12.3    8 x 32 + 500   14.9 / 18.9   8 x 64 + 500   16.8 / 33.5
+//           2 x 64          9.0 / 7.1     8 x 64          9.2 / 12.7   1 x 1000 + 4000  92 / 343
+//           1 x 16 + 8000  26.1 / 18.2    1 x 32 + 8000  26.8 / 28.0   1 x 64 + 8000  29.0 / 48.9
+//   fp16    1 x 64 + 500   14.9 / 13.1    1 x 128 + 500  15.1 / 14.1   1 x 256 + 500  16.6 / 24.1
+//           8 x 16 + 500   16.6 / 13.3    8 x 32 + 500   17.5 / 20.5   8 x 64 + 500   19.4 / 39.7
+//           1 x 32 + 8000  39.5 / 29.3    1 x 64 + 8000  41.5 / 49.2   1 x 1000 + 4000 160 / 351
 inline bool use_chunk_kernel(const WinParams& p) {
+    static const int forced = [] {
+        const char* v = getenv("QTTS_WINDOW_TILES");
+        return v && (v[0] == '0' || v[0] == '1') ? v[0] - '0' : -1;
+    }();
     if (p.S < 2 || p.group > 128) return false;
     if (((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_lo)) & 15) != 0) return false;
-    return p.S * p.group >= 32;
+    if (forced >= 0) return forced == 1;
+    const long long heads = (long long)(p.R / p.S) * p.kv_heads, rows = (long long)p.S * p.group;
+    if (rows < 64 || (rows < 128 && heads < 16)) return false;
+    const long long row_tiles = heads * (p.group >= 8 ? (long long)p.S * ceil_div(p.group, 8) : ceil_div(p.S, 8 / p.group));
+    long long keys = p.max_ctx;
+    if (p.window > 0 && (long long)p.window + p.sinks + 32 < keys) keys = (long long)p.window + p.sinks + 32;
+    return row_tiles > 4 * num_sms() || row_tiles * (keys / 16) >= 8192;
 }
 
 template <int FMT, int D>

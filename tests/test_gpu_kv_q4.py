@@ -15,6 +15,8 @@ roundings conspire; as they are independent, the root mean square over a row is 
 expectation's bound as well: (d2 + 2^-11) rms(v) with d2 = 2^-11 |q| max|k| / D (times sqrt 2 at 4 bits)."""
 
 
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -259,7 +261,9 @@ def _attend(fmt, *a, window=0, sinks=0, **kw):
 
 
 def _is_chunk(S, Hq, H):
-    return S > 1 and S * Hq // H >= 32
+    """Whether rows may go through fp16 tiles."""
+    forced = os.environ.get("QTTS_WINDOW_TILES")
+    return S > 1 and forced != "0" and (forced == "1" or S * Hq // H >= 64)
 
 
 def _tolerance(fmt, q, kv, chunk=False):
@@ -360,6 +364,29 @@ def test_long_chunks(fmt, S):
     _run_case(fmt, 4, 2, 128, [S + 37, S], S, 0, 0, seed=S)
     _run_case(fmt, 4, 2, 128, [S + 203], S, 65, 7, seed=S)
     _run_case(fmt, 8, 2, 64, [S + 9], S, 0, 0, seed=S)
+
+
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
+def test_many_chunks(fmt):
+    """Enough rows for the tile kernel by its own rule, several CTAs a tile and one."""
+    _run_case(fmt, 16, 8, 128, [300, 150], 150, 0, 0)
+    _run_case(fmt, 16, 8, 128, [1300], 100, 0, 0)
+    _run_case(fmt, 16, 8, 128, [400, 210, 333, 205, 50], 200, 100, 20)
+
+
+@pytest.mark.skipif(os.environ.get("QTTS_WINDOW_TILES") is not None, reason="already a forced run")
+@pytest.mark.parametrize("form", ["0", "1"])
+def test_both_chunk_forms(form):
+    """Chunks go through 8-row or 128-row tiles by a rule on their sizes (QTTS_WINDOW_TILES forces one, read
+    once per process): rerun every chunk case in a child process with each."""
+    import subprocess
+    import sys
+
+    env = dict(os.environ, QTTS_WINDOW_TILES=form)
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k",
+                        "chunk or reach", os.path.abspath(__file__)], env=env, capture_output=True, text=True,
+                       timeout=900)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
