@@ -231,7 +231,8 @@ int qtts_paged_attention_noalloc(const void* q, int R, int num_heads, int kv_hea
 /* Quantise the K and V rows of n tokens and n_layers layers (from first_layer) into the pool
  * positions slot_mapping[n] (block * 16 + offset; negative or past the pool: skipped), as the
  * tokens of a step are written.  k, v: elements of `dtype` (QTTS_F16 / BF16 / F32), channels
- * contiguous; k_strides, v_strides: element strides of (token, layer, head), host arrays of 3.
+ * contiguous; k_strides, v_strides: element strides of (token, layer, head), host arrays of 3, each
+ * in [0, 2^31).
  * The positions of one call must differ: of two tokens written to one position, the cache keeps a
  * mixture. */
 int qtts_kv_write_q4(void* cache, int num_blocks, int num_layers, int kv_heads, int head_dim, const void* k,

@@ -16,6 +16,8 @@
 // lane channels of every group.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace qtts {
@@ -50,7 +52,8 @@ struct Q4IoParams {
     uint8_t* cache;
     const void *k_in, *v_in;            // write: rows in
     void *k_out, *v_out;                // read: rows out
-    long long ks[3], vs[3];             // element strides of (token, layer, head)
+    int ks[3], vs[3];                   // element strides of (token, layer, head)
+    uint32_t block_bytes;               // of a pool block
     int num_blocks, num_layers, kv_heads, first_layer;
     int n;                              // tokens
     const int32_t* mapping;             // position of each token (block * 16 + offset) ...
@@ -89,6 +92,37 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// Smallest and largest of a group's 64 values, eight in each of the row's eight threads; NaN if any is.
+// 16-bit types go two to an instruction, and as the pair (min, -max) through the shuffles.
+template <typename T>
+__device__ __forceinline__ float2 group_range(const T (&x)[8], unsigned peers) {
+    if constexpr (sizeof(T) == 4) {
+        float lo = x[0], hi = x[0];
+#pragma unroll
+        for (int c = 1; c < 8; ++c) lo = min_nan(lo, x[c]), hi = max_nan(hi, x[c]);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            lo = min_nan(lo, __shfl_xor_sync(peers, lo, o));
+            hi = max_nan(hi, __shfl_xor_sync(peers, hi, o));
+        }
+        return make_float2(lo, hi);
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2* v = reinterpret_cast<const T2*>(x);
+        const T2 mn = __hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3]));
+        const T2 mx = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+        T2 r;
+        r.x = __hmin_nan(mn.x, mn.y);
+        r.y = __hneg(__hmax_nan(mx.x, mx.y));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            const uint32_t u = __shfl_xor_sync(peers, *reinterpret_cast<const uint32_t*>(&r), o);
+            r = __hmin2_nan(r, *reinterpret_cast<const T2*>(&u));
+        }
+        return make_float2(q4_to_float<T>(r.x), -q4_to_float<T>(r.y));
+    }
+}
+
 // Where thread group `flat` works: rows are ordered 16 tokens innermost, then head, k|v, layer, then
 // the next 16 tokens, so that consecutive rows of a whole block fill a chunk.
 struct Q4Row {
@@ -116,8 +150,25 @@ __device__ __forceinline__ uint8_t* q4_chunk(const Q4IoParams& p, const Q4Row& r
         *off = r.token & 15;
     }
     if (blk < 0 || blk >= p.num_blocks) return nullptr;
-    const size_t c = (((size_t)blk * p.num_layers + p.first_layer + r.layer) * 2 + r.kv) * p.kv_heads + r.head;
-    return p.cache + c * Q4Layout<D>::CHUNK;
+    const uint32_t in_block = (uint32_t)(((p.first_layer + r.layer) * 2 + r.kv) * p.kv_heads + r.head) * Q4Layout<D>::CHUNK;
+    return p.cache + (uint64_t)(uint32_t)blk * p.block_bytes + in_block;
+}
+
+// Element offset of a row from its K or V base.
+__device__ __forceinline__ long long q4_offset(const Q4IoParams& p, const Q4Row& r) {
+    const int st0 = r.kv ? p.vs[0] : p.ks[0], st1 = r.kv ? p.vs[1] : p.ks[1], st2 = r.kv ? p.vs[2] : p.ks[2];
+    return (long long)r.token * st0 + (long long)r.layer * st1 + (long long)r.head * st2;
+}
+
+// The code of d = x - zero by exact remainders; rare, and so a call.
+__device__ __noinline__ float q4_exact_code(float d, float scale, float inv15) {
+    float k = rintf(__saturatef(d * inv15) * 15.f);
+    // e = d - k scale is exact wherever it is near scale / 2
+    const float e = __fmaf_rn(-k, scale, d), h = 0.5f * scale;
+    const bool odd = (int)k & 1;
+    if (e > h || (e == h && odd)) k += 1.f;
+    else if (e < -h || (e == -h && odd)) k -= 1.f;
+    return fminf(fmaxf(k, 0.f), 15.f);
 }
 
 // Eight threads a row, thread i taking the channels 64 w + 8 i .. + 7 of every group w.
@@ -134,10 +185,8 @@ __global__ void __launch_bounds__(256) kv_write_q4_kernel(const Q4IoParams p) {
     uint8_t* chunk = in_range && r.token < p.n ? q4_chunk<D>(p, r, &off) : nullptr;
     const unsigned peers = 0xffu << (threadIdx.x & 24);  // the row's eight threads go together
     if (!chunk) return;
-    const long long* st = r.kv ? p.vs : p.ks;
-    const T* src = reinterpret_cast<const T*>(r.kv ? p.v_in : p.k_in) + r.token * st[0] + r.layer * st[1] +
-                   r.head * st[2] + 8 * i;
-    T x[L::NG][8];
+    const T* src = reinterpret_cast<const T*>(r.kv ? p.v_in : p.k_in) + q4_offset(p, r) + 8 * i;
+    __align__(16) T x[L::NG][8];
 #pragma unroll
     for (int w = 0; w < L::NG; ++w) {
         if constexpr (VEC) {
@@ -152,56 +201,44 @@ __global__ void __launch_bounds__(256) kv_write_q4_kernel(const Q4IoParams p) {
     uint32_t word[L::NG];
 #pragma unroll
     for (int w = 0; w < L::NG; ++w) {
-        float f[8], lo, hi;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            f[c] = q4_to_float<T>(x[w][c]);
-            lo = c ? min_nan(lo, f[c]) : f[c];
-            hi = c ? max_nan(hi, f[c]) : f[c];
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            lo = min_nan(lo, __shfl_xor_sync(peers, lo, o));
-            hi = max_nan(hi, __shfl_xor_sync(peers, hi, o));
-        }
-        const bool nan = lo != lo;
-        lo = __fadd_rn(fminf(fmaxf(lo, -65504.f), 65504.f), 0.f);  // of zeros of both signs, +0
-        hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+        const float2 range = group_range<T>(x[w], peers);
+        const bool nan = range.x != range.x;
+        // of zeros of both signs, +0
+        const float lo = __fadd_rn(fminf(fmaxf(range.x, -65504.f), 65504.f), 0.f);
+        const float hi = fminf(fmaxf(range.y, -65504.f), 65504.f);
         const __half zero_h = nan ? __ushort_as_half(0x7fff) : __float2half_rn(lo);
         const __half scale_h = nan ? __float2half_rn(0.f)
                                    : __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
         const float zero = __half2float(zero_h), scale = __half2float(scale_h);
-        // t = quotient / 15, saturated to [0, 1] (NaN -> 0), then 15 t rounded to an integer by
-        // adding 2^23 + 2^22: its bits hold the code.  The reciprocal puts 15 t off by at most
-        // 2^-19; where it lands that close to a border the code is decided by exact remainders.
-        constexpr float kMagic = 12582912.f;  // 0x4B400000
-        const float inv15 = scale > 0.f ? __frcp_rn(scale) * (1.0f / 15.0f) : 0.f;
-        uint32_t acc = 0;
-        float worst = 0.f;
-        float d[8];
+        // t = (x - zero) / (15 scale), saturated to [0, 1] (NaN -> 0), then 15 t rounded to an integer
+        // by adding 2^23 + 2^22.  The approximate reciprocal (2^-23) and the product that x - zero is folded
+        // into put 15 t off by at most 5.4e-6 + 2^-24 |zero| / scale; where it lands within that (and a
+        // margin) of a border the code is decided by exact remainders.
+        constexpr float kMagic = 12582912.f;
+        const float inv = scale > 0.f ? __fdividef(1.f, scale) : 0.f, inv15 = inv * (1.0f / 15.0f), shift = -zero * inv15;
+        const float near = 0.5f - (8e-6f + 2.4e-7f * fabsf(zero) * inv);
+        float code[8], worst = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            d[c] = __fsub_rn(f[c], zero);
-            const float t = __saturatef(d[c] * inv15);
-            const float m = __fmaf_rn(t, 15.f, kMagic);
-            worst = fmaxf(worst, fabsf(__fmaf_rn(t, 15.f, kMagic - m)));
-            acc += __float_as_uint(m) << (4 * c);
+            const float t = __saturatef(__fmaf_rn(q4_to_float<T>(x[w][c]), inv15, shift));
+            code[c] = __fmaf_rn(t, 15.f, kMagic) - kMagic;
+            worst = fmaxf(worst, fabsf(__fmaf_rn(t, 15.f, -code[c])));
         }
-        acc -= 0x3F400000u;  // what the constant's own bits added up to, modulo 2^32
-        if (worst > 0.499995f) {
-            acc = 0;
+        if (worst > near) {  // about one value in 2500 of a normal fp16 row lies exactly on a border
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                const float t = __saturatef(d[c] * inv15);
-                int code = (int)rintf(t * 15.f);
-                // e = d - code * scale is exact wherever it is near scale / 2
-                const float e = __fmaf_rn(-(float)code, scale, d[c]), h = 0.5f * scale;
-                const bool odd = code & 1;
-                if (e > h || (e == h && odd)) ++code;
-                else if (e < -h || (e == -h && odd)) --code;
-                acc |= (uint32_t)min(max(code, 0), 15) << (4 * c);
+                const float t = __saturatef(__fmaf_rn(q4_to_float<T>(x[w][c]), inv15, shift));
+                if (fabsf(__fmaf_rn(t, 15.f, -code[c])) > near)
+                    code[c] = q4_exact_code(__fsub_rn(q4_to_float<T>(x[w][c]), zero), scale, inv15);
             }
         }
+        // four codes to an exact 16-bit integer in fp32, two of those to a word
+        float half_word[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            half_word[h] = __fmaf_rn(__fmaf_rn(__fmaf_rn(code[4 * h + 3], 16.f, code[4 * h + 2]), 16.f, code[4 * h + 1]), 16.f,
+                                     code[4 * h]) + kMagic;
+        const uint32_t acc = __byte_perm(__float_as_uint(half_word[0]), __float_as_uint(half_word[1]), 0x5410);
         word[w] = acc;
         if (i == w)  // one thread of the row writes each group's parameters
             *reinterpret_cast<__half2*>(chunk + L::PARAMS + w * 64 + off * 4) = __halves2half2(scale_h, zero_h);
@@ -223,9 +260,7 @@ __global__ void __launch_bounds__(256) kv_read_q4_kernel(const Q4IoParams p) {
     if (r.token >= p.n) return;
     int off = 0;
     const uint8_t* chunk = q4_chunk<D>(p, r, &off);
-    const long long* st = r.kv ? p.vs : p.ks;
-    T* dst = reinterpret_cast<T*>(r.kv ? p.v_out : p.k_out) + r.token * st[0] + r.layer * st[1] + r.head * st[2] +
-             8 * i;
+    T* dst = reinterpret_cast<T*>(r.kv ? p.v_out : p.k_out) + q4_offset(p, r) + 8 * i;
     uint32_t word[L::NG] = {};
     __half2 prm[L::NG];
 #pragma unroll
@@ -245,11 +280,31 @@ __global__ void __launch_bounds__(256) kv_read_q4_kernel(const Q4IoParams p) {
     }
 #pragma unroll
     for (int w = 0; w < L::NG; ++w) {
-        const float scale = __low2float(prm[w]), zero = __high2float(prm[w]);
-        T y[8];
+        __align__(16) T y[8];
+        if constexpr (std::is_same<T, __half>::value) {
+            // 1024 + code and 1024 + 16 code are fp16 numbers with the nibble in their low bits; code * scale
+            // + zero is then one rounding of the exact value
+            const __half2 scale = __low2half2(prm[w]), zero = __high2half2(prm[w]);
+            const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
+                          k64 = __floats2half2_rn(-64.f, -64.f);
+            uint32_t v[4];  // channels (0, 4), (1, 5), (2, 6), (3, 7)
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            y[c] = q4_from_float<T>(__fmaf_rn((float)((word[w] >> (4 * c)) & 15u), scale, zero));
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t u = word[w] >> (8 * h);
+                const uint32_t a = (u & 0x000f000fu) | 0x64006400u, b = (u & 0x00f000f0u) | 0x64006400u;
+                const __half2 va = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&a), k1024), scale, zero);
+                const __half2 vb = __hfma2(__hfma2(*reinterpret_cast<const __half2*>(&b), k16, k64), scale, zero);
+                v[2 * h] = *reinterpret_cast<const uint32_t*>(&va);
+                v[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&vb);
+            }
+            *reinterpret_cast<uint4*>(y) = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                                      __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+        } else {
+            const float scale = __low2float(prm[w]), zero = __high2float(prm[w]);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                y[c] = q4_from_float<T>(__fmaf_rn((float)((word[w] >> (4 * c)) & 15u), scale, zero));
+        }
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < (int)sizeof(T) / 2; ++c)
@@ -262,10 +317,10 @@ __global__ void __launch_bounds__(256) kv_read_q4_kernel(const Q4IoParams p) {
 }
 
 // 16-byte accesses: the base and every stride must keep rows 16-byte aligned
-inline bool q4_vec_ok(const void* k, const void* v, const long long* ks, const long long* vs, int elem) {
+inline bool q4_vec_ok(const void* k, const void* v, const int* ks, const int* vs, int elem) {
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return false;
     for (int s = 0; s < 3; ++s)
-        if ((ks[s] * elem) & 15 || (vs[s] * elem) & 15) return false;
+        if (((unsigned)ks[s] * elem) & 15 || ((unsigned)vs[s] * elem) & 15) return false;
     return true;
 }
 
@@ -287,6 +342,9 @@ template <bool WRITE>
 inline int run_q4_io(Q4IoParams p, int layers, int head_dim, int dtype, cudaStream_t st) {
     const long long per_token = (long long)layers * 2 * p.kv_heads;
     QTTS_REQUIRE(per_token <= (1 << 20), "q4 cache: %lld rows per token", per_token);
+    const long long block_bytes = (long long)p.num_layers * 2 * p.kv_heads * 9 * head_dim;
+    QTTS_REQUIRE(block_bytes < (1ll << 31), "q4 cache: %lld bytes per block", block_bytes);
+    p.block_bytes = (uint32_t)block_bytes;
     p.rows = make_fastdiv((uint32_t)per_token);
     p.heads = make_fastdiv((uint32_t)p.kv_heads);
     // row numbers stay below 2^31: longer inputs go in several launches

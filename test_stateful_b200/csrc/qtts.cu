@@ -46,6 +46,9 @@ static int q4_io_check(const char* what, const void* cache, int num_blocks, int 
     QTTS_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0 && (reinterpret_cast<uintptr_t>(index) & 3) == 0 &&
                      ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & (elem - 1)) == 0,
                  "%s: misaligned pointer", what);
+    for (int i = 0; i < 3; ++i)
+        QTTS_REQUIRE(ks[i] >= 0 && vs[i] >= 0 && ks[i] < (1ll << 31) && vs[i] < (1ll << 31),
+                     "%s: strides must be in [0, 2^31) elements", what);
     return QTTS_OK;
 }
 
@@ -58,7 +61,7 @@ static Q4IoParams q4_io_params(const void* cache, int num_blocks, int num_layers
     p.kv_heads = kv_heads;
     p.first_layer = first_layer;
     p.n = n;
-    for (int i = 0; i < 3; ++i) p.ks[i] = ks[i], p.vs[i] = vs[i];
+    for (int i = 0; i < 3; ++i) p.ks[i] = (int)ks[i], p.vs[i] = (int)vs[i];
     return p;
 }
 
