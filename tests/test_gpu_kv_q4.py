@@ -358,6 +358,28 @@ def test_long_rows_split_over_a_cluster(fmt, ctx):
     _run_case(fmt, 4, 2, 64, [ctx, 17], 1, 3000, 4)
 
 
+def test_long_rows_are_unbiased():
+    """Nearly uniform attention over zero-mean values: 4-bit values are code * scale + zero, two sums of some 7.5
+    scales that cancel to a few hundredths, so a rounding of p * scale in one direction would show.  To
+    nearest, a term is off by 2^-17 of at most 15 scale / n, 9001 of them at random 15 * 2^-17 / sqrt(3 n) =
+    7e-7 scale; fp32 sums of some 10 blocks a warp, 10 * 2^-24 * 7.5 = 4.5e-6 scale at most; the output
+    2^-17 of itself: together below 2^-16 scale in the root mean square (cutting p off: 6e-5)."""
+    H, D, ctx = 2, 128, 9001
+    nb = -(-ctx // 16)
+    x = torch.randn(nb, 1, 2, H, 16, D, generator=_gen(3)).half().float().numpy()
+    raw = O.pack(*O.quantise(x))
+    scale = O.quantise(x[:, 0, 1])[1].astype(np.float64).max()
+    vals = O.unpack(raw)[:, 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
+    q = torch.randn(1, 4, D, generator=_gen(4)) * 0.01
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    lo = torch.empty(1, 4 * D, device=DEV, dtype=torch.bfloat16)
+    out = ops.paged_attention_q4(q.to(DEV), torch.from_numpy(raw).to(DEV), 0,
+                                 torch.arange(nb, dtype=torch.int32, device=DEV).view(1, nb), zero, zero + ctx, nb * 16,
+                                 out_lo=lo)
+    err = (out.double() + lo.double()).cpu().numpy()[0] - O.attention(q[0].numpy(), vals[0], vals[1], ctx)
+    assert np.sqrt((err ** 2).mean()) < 2.0 ** -16 * scale
+
+
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
 @pytest.mark.parametrize("S", [100, 300])
 def test_long_chunks(fmt, S):
