@@ -4,11 +4,16 @@
     python microbench.py prefill-attention [--streams 8] [--prefill-chunk 128] [--past 384]
     python microbench.py gemm [--n 12288] [--k 2048] [--m 64] [--launches 50]
     python microbench.py code2wav [--rows 64] [--launches 50] [--chunk 25]
+    python microbench.py window-attention [--kv fp16|q4] [--rows 64] [--ctx-mean 520] [--window 0] [--sinks 0]
+                                          [--rows-per-stream 1]
+    python microbench.py kv-q4 [--tokens 501]
 
 Prints one JSON line with the mean launch time (CUDA events) and the
 achieved bandwidth over the kernel's algorithmic bytes:
 * attention: K+V bytes of every visible key of one layer (fp16) + q/out;
-* gemm: the weight bytes (bf16) + activation hi/lo operands + fp32 output.
+* gemm: the weight bytes (bf16) + activation hi/lo operands + fp32 output;
+* window-attention: K+V bytes of every key some row of a stream sees (fp16 or 4.5 bits) + q/out;
+* kv-q4: 28 layers of a prompt's K/V quantised into a 4-bit pool, then read back (fp16 rows + pool bytes, each way).
 Inputs cycle through enough copies that every launch reads from HBM.  The
 same command is the small case for an ``ncu --set full`` capture.
 """
@@ -138,6 +143,80 @@ def bench_prefill_attention(streams: int, chunk: int, past: int, launches: int, 
             "decode_kernel_same_rows_us": t_dec * 1e6, "speedup_vs_decode_rows": t_dec / t_pre}
 
 
+def _graph_time(launch, launches: int) -> float:
+    """Seconds per call of ``launch(i)``, captured in a CUDA graph (the host path is not timed)."""
+    for i in range(3):
+        launch(i)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            for i in range(launches):
+                launch(i)
+        graph.replay()
+        s.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record(s)
+        graph.replay()
+        e1.record(s)
+        s.synchronize()
+    return e0.elapsed_time(e1) / 1e3 / launches
+
+
+def bench_window_attention(fmt: str, rows: int, rows_per_stream: int, ctx_mean: int, spread: float, window: int,
+                           sinks: int, launches: int, layers: int = 4, seed: int = 0):
+    """Windowed attention over the fp16 pool or the 4-bit one: ``rows`` streams of ``rows_per_stream``
+    consecutive rows, contexts U[mean (1 - spread), mean (1 + spread)]."""
+    dev = "cuda"
+    g = torch.Generator().manual_seed(seed)
+    S = rows_per_stream
+    lo, hi = max(S, int(ctx_mean * (1 - spread))), max(S, int(ctx_mean * (1 + spread)))
+    ctx = torch.randint(lo, hi + 1, (rows,), generator=g)
+    mbps = -(-hi // 16)
+    total = rows * mbps
+    if fmt == "q4":
+        pool = torch.zeros(total, layers, 2, 8, 9 * 128, dtype=torch.uint8, device=dev)
+        m = torch.arange(total * 16, dtype=torch.int32, device=dev)
+        for l in range(layers):
+            kv = torch.randn(2, total * 16, 8, 128, device=dev, dtype=torch.float16)
+            ops.kv_write_q4(pool, kv[0], kv[1], m, layer=l)
+    else:
+        pool = torch.randn(total, layers, 2, 8, 16, 128, device=dev, dtype=torch.float16)
+    table = torch.randperm(total, generator=g).to(torch.int32).view(rows, mbps).to(dev)
+    q = torch.randn(rows * S, 16, 128, generator=g).to(dev)
+    row_slot = torch.arange(rows, dtype=torch.int32).repeat_interleave(S).to(dev)
+    row_ctx = (ctx[:, None] - S + 1 + torch.arange(S)[None, :]).flatten().to(torch.int32).to(dev)
+    out = torch.empty(rows * S, 16 * 128, device=dev, dtype=torch.bfloat16)
+    attend = ops.paged_attention_q4 if fmt == "q4" else ops.paged_attention_window
+    sec = _graph_time(lambda i: attend(q, pool, i % layers, table, row_slot, row_ctx, mbps * 16, window=window,
+                                       sinks=sinks, rows_per_stream=S, out=out), launches)
+    w = window or 1 << 30
+    keys = sum(min(c, min(c, w + S - 1) + min(sinks, max(0, c - w - S + 1))) for c in ctx.tolist())
+    algo = keys * 2 * 8 * (72 if fmt == "q4" else 256) + rows * S * 16 * 128 * (4 + 2)
+    return {"kernel": "paged attention, window + sinks", "kv": fmt, "streams": rows, "rows_per_stream": S,
+            "window": window, "sinks": sinks, "keys": keys, "launch_us": sec * 1e6, "algorithmic_bytes": algo,
+            "achieved_gbs": algo / sec / 1e9}
+
+
+def bench_kv_q4(tokens: int, launches: int, layers: int = 28):
+    dev = "cuda"
+    sets = max(2, -(-300_000_000 // (tokens * layers * 2 * 8 * 128 * 2)))  # > 2x L2 of distinct rows
+    nb = -(-tokens // 16)
+    kv = [torch.randn(tokens, layers, 2, 8, 128, device=dev, dtype=torch.float16) for _ in range(sets)]
+    pool = torch.zeros(nb, layers, 2, 8, 9 * 128, dtype=torch.uint8, device=dev)
+    m = torch.randperm(nb * 16)[:tokens].sort().values.to(torch.int32).to(dev)
+    outs = [torch.empty(2, tokens, layers, 8, 128, device=dev, dtype=torch.float16) for _ in range(sets)]
+    t_w = _graph_time(lambda i: ops.kv_write_q4(pool, kv[i % sets][:, :, 0], kv[i % sets][:, :, 1], m), launches)
+    t_r = _graph_time(lambda i: ops.kv_read_q4(pool, m, n_layers=layers, k=outs[i % sets][0], v=outs[i % sets][1]),
+                      launches)
+    values = tokens * layers * 2 * 8 * 128
+    algo = values * 2 + values // 2 + values // 16
+    return {"kernel": "kv_write_q4_kernel / kv_read_q4_kernel", "tokens": tokens, "layers": layers,
+            "write_us": t_w * 1e6, "read_us": t_r * 1e6, "algorithmic_bytes_each": algo,
+            "write_gbs": algo / t_w / 1e9, "read_gbs": algo / t_r / 1e9}
+
+
 def bench_gemm(n: int, k: int, m: int, launches: int, seed: int = 0, plain: bool = False):
     dev = "cuda"
     g = torch.Generator(device=dev).manual_seed(seed)
@@ -221,7 +300,7 @@ def bench_code2wav(rows: int, launches: int, seed: int = 0, chunk: int = 1):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["attention", "prefill-attention", "gemm", "code2wav"])
+    ap.add_argument("what", choices=["attention", "prefill-attention", "gemm", "code2wav", "window-attention", "kv-q4"])
     ap.add_argument("--streams", type=int, default=8, help="prefill-attention: streams with one chunk each")
     ap.add_argument("--prefill-chunk", type=int, default=128, help="prefill-attention: query rows per stream")
     ap.add_argument("--past", type=int, default=384, help="prefill-attention: positions before the chunk")
@@ -233,6 +312,11 @@ def main():
     ap.add_argument("--m", type=int, default=64)
     ap.add_argument("--launches", type=int, default=50)
     ap.add_argument("--split", type=int, default=0, help="attention: KV blocks per split (0: library default)")
+    ap.add_argument("--kv", choices=["fp16", "q4"], default="fp16", help="window-attention: pool format")
+    ap.add_argument("--window", type=int, default=0, help="window-attention: keys a row looks back (0: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="window-attention: first keys that stay visible")
+    ap.add_argument("--rows-per-stream", type=int, default=1, help="window-attention: consecutive rows of a stream")
+    ap.add_argument("--tokens", type=int, default=501, help="kv-q4: tokens written and read")
     ap.add_argument("--chunk", type=int, default=1, help="code2wav: frames per stream per call")
     ap.add_argument("--plain", action="store_true", help="gemm: plain bf16 activations (no lo operand)")
     a = ap.parse_args()
@@ -240,6 +324,11 @@ def main():
         r = bench_attention(a.rows, a.ctx_mean, a.launches, split=a.split, spread=a.ctx_spread)
     elif a.what == "prefill-attention":
         r = bench_prefill_attention(a.streams, a.prefill_chunk, a.past, a.launches, split=a.split)
+    elif a.what == "window-attention":
+        r = bench_window_attention(a.kv, a.rows, a.rows_per_stream, a.ctx_mean, a.ctx_spread, a.window, a.sinks,
+                                   a.launches)
+    elif a.what == "kv-q4":
+        r = bench_kv_q4(a.tokens, a.launches)
     elif a.what == "code2wav":
         r = bench_code2wav(a.rows, a.launches, chunk=a.chunk)
     else:
