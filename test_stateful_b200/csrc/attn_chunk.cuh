@@ -108,20 +108,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
 #pragma unroll
     for (int k = 0; k < 12; ++k) {
         float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (warp < 12 && q_row(k) < rows) u = __ldg(reinterpret_cast<const float4*>(p.q + head_row(q_row(k)) * D) + lane % LPR);
+        if (warp < 12 && q_row(k) < rows) u = __ldcg(reinterpret_cast<const float4*>(p.q + head_row(q_row(k)) * D) + lane % LPR);
         if (k < 6) q_now[k] = u;
         else q_next[k - 6] = u;
     }
     const int limit = min(p.max_ctx, p.mbps * 16);
     const int window = p.window > 0 ? p.window : 0x7fffffff;
-    const int slot = __ldg(p.row_slot + row0);
+    const int slot = __ldcg(p.row_slot + row0);
     const bool slot_ok = slot >= 0 && slot < p.num_slots;
     if (!slot_ok && threadIdx.x == 0) record_error(DEV_ERR_ATTN_BOUNDS);
 
     const int r = threadIdx.x;  // softmax threads: the row
     int ctx = 0;
     if (warp < 4) {
-        if (r < rows && slot_ok) ctx = min(max(__ldg(p.row_ctx + row0 + p.by_group.div(r)), 0), limit);
+        if (r < rows && slot_ok) ctx = min(max(__ldcg(p.row_ctx + row0 + p.by_group.div(r)), 0), limit);
         int hi = ctx, lo = ctx > 0 ? ctx : 0x7fffffff;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) {
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             const int pos = (t0 + i + lane) * 4 + w4;
             ids = -1;
             if (i + lane < nt && pos < nb) {
-                ids = __ldg(table + (first_key(pos) >> 4));
+                ids = __ldcg(table + (first_key(pos) >> 4));
                 if (ids < 0 || ids >= p.num_blocks) {
                     record_error(DEV_ERR_ATTN_BOUNDS);
                     ids = -1;

@@ -215,15 +215,15 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
             const float* qr = p.q + ((size_t)(row0 + s / heads) * p.num_heads + kvh * p.group + h0 + s % heads) * D;
             if constexpr (FMT == kWinQ4) {
                 if (lane < 16 * NW) {
-                    const float4 a = __ldg(reinterpret_cast<const float4*>(qr + 8 * (lane >> 1)));
-                    const float4 b = __ldg(reinterpret_cast<const float4*>(qr + 8 * (lane >> 1) + 4));
+                    const float4 a = __ldcg(reinterpret_cast<const float4*>(qr + 8 * (lane >> 1)));
+                    const float4 b = __ldcg(reinterpret_cast<const float4*>(qr + 8 * (lane >> 1) + 4));
                     qv[k][0] = lane & 1 ? a.y : a.x, qv[k][1] = lane & 1 ? a.w : a.z;
                     qv[k][2] = lane & 1 ? b.y : b.x, qv[k][3] = lane & 1 ? b.w : b.z;
                 }
             } else {
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
-                    const float2 a = __ldg(reinterpret_cast<const float2*>(qr) + lane + 32 * w);
+                    const float2 a = __ldcg(reinterpret_cast<const float2*>(qr) + lane + 32 * w);
                     qv[k][2 * w] = a.x, qv[k][2 * w + 1] = a.y;
                 }
             }
@@ -233,14 +233,14 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     // contexts: this lane's score columns, and the tile's extremes over rows that see anything
     const int limit = min(p.max_ctx, p.mbps * 16);
     const int window = p.window > 0 ? p.window : 0x7fffffff;
-    const int slot = __ldg(p.row_slot + row0);
+    const int slot = __ldcg(p.row_slot + row0);
     const bool slot_ok = slot >= 0 && slot < p.num_slots;
     int ctx[2];
     int cmax = 0, cmin = 0x7fffffff;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int s = (2 * t + e) % SL;
-        ctx[e] = s < slots && slot_ok ? min(max(__ldg(p.row_ctx + row0 + s / heads), 0), limit) : 0;
+        ctx[e] = s < slots && slot_ok ? min(max(__ldcg(p.row_ctx + row0 + s / heads), 0), limit) : 0;
         cmax = max(cmax, ctx[e]);
         if (ctx[e] > 0) cmin = min(cmin, ctx[e]);
     }
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     bool bad_id = false;  // an id outside the pool came up: its keys are hidden
     auto table_id = [&](int n) {  // of the warp's block n
         const int i = i0 + n;
-        return __ldg(table + (i < nb_sink ? i : i + past_sinks));
+        return __ldcg(table + (i < nb_sink ? i : i + past_sinks));
     };
     // copy the K (v = 0) or V chunks of blocks n .. n + KB - 1; every lane commits a group, full or empty
     auto issue = [&](int n, int v, uint32_t buf) {

@@ -62,6 +62,8 @@ struct Q4IoParams {
     uint32_t total;                     // ceil(n / 16) * 16 * rows
 };
 
+// Inputs are read through L2 (__ldcg): a kernel launched with programmatic dependent launch begins
+// before its predecessor has written them, so they are not read-only for the kernel's life.
 template <typename T>
 __device__ __forceinline__ float q4_to_float(T x);
 template <>
@@ -142,12 +144,12 @@ template <int D>
 __device__ __forceinline__ uint8_t* q4_chunk(const Q4IoParams& p, const Q4Row& r, int* off) {
     int blk;
     if (p.mapping) {
-        const int m = __ldg(p.mapping + r.token);
+        const int m = __ldcg(p.mapping + r.token);
         if (m < 0) return nullptr;
         blk = m >> 4;
         *off = m & 15;
     } else {
-        blk = __ldg(p.blocks + (r.token >> 4));
+        blk = __ldcg(p.blocks + (r.token >> 4));
         *off = r.token & 15;
     }
     if (blk < 0 || blk >= p.num_blocks) return nullptr;
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kQ4Threads) kv_write_q4_kernel(const Q4IoParam
             if constexpr (VEC) {
                 const uint4* s4 = reinterpret_cast<const uint4*>(src + 64 * w + 32 * h);
 #pragma unroll
-                for (int c = 0; c < (int)sizeof(T) / 2; ++c) reinterpret_cast<uint4*>(x[w] + 8 * h)[c] = __ldg(s4 + c);
+                for (int c = 0; c < (int)sizeof(T) / 2; ++c) reinterpret_cast<uint4*>(x[w] + 8 * h)[c] = __ldcg(s4 + c);
             } else {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) x[w][8 * h + c] = src[64 * w + 32 * h + c];
