@@ -186,6 +186,8 @@ def kv_write_q4(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapp
     _need_i32("slot_mapping", slot_mapping, 1)
     n = slot_mapping.shape[0]
     layers, dt, ks = _q4_rows("k", k, n, None, H, D)
+    if layer < 0 or not 1 <= layers <= L - layer:
+        raise ValueError(f"kv_write_q4: layers [{layer}, +{layers}) of {L}")
     _, vdt, vs = _q4_rows("v", v, n, layers, H, D)
     if dt != vdt:
         raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
@@ -214,6 +216,9 @@ def kv_read_q4(cache: torch.Tensor, slot_mapping: torch.Tensor, layer: int = 0, 
     _, vdt, vs = _q4_rows("v", v, n, n_layers, H, D)
     if dt != vdt:
         raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
+    for st in (ks, vs):
+        if (n > 1 and not st[0]) or (n_layers > 1 and k.dim() == 4 and not st[1]) or (H > 1 and not st[2]):
+            raise ValueError("kv_read_q4: k and v must not be broadcast tensors")
     _launch(dev, "kv_read_q4", _lib.load().qtts_kv_read_q4, cache.data_ptr(), nb, L, H, D, k.data_ptr(), v.data_ptr(), dt,
             ks, vs, layer, n_layers, slot_mapping.data_ptr(), n)
     return k, v
@@ -250,6 +255,10 @@ def _window_attention(what, fn, q, kv, dims, layer, block_table, row_slot, row_c
     _need_i32("row_slot", row_slot, 1)
     _need_i32("row_ctx", row_ctx, 1)
     slots, mbps = block_table.shape
+    if not (0 <= layer < L and 0 < max_ctx <= 16 * mbps and 0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
+        raise ValueError(f"{what}: layer {layer} of {L}, max_ctx {max_ctx} of {16 * mbps}, window {window}, sinks {sinks}")
+    if rows_per_stream < 1 or R % rows_per_stream:
+        raise ValueError(f"{what}: {R} rows are not streams of {rows_per_stream} tokens")
     if row_slot.shape[0] != R or row_ctx.shape[0] != R:
         raise ValueError(f"{what}: {R} query rows, {row_slot.shape[0]} slots and {row_ctx.shape[0]} contexts")
     if out is None:

@@ -232,6 +232,15 @@ def test_wrapper_refusals_on_device():
            lambda: ops.paged_attention_q4(q, cache, 0, t, two[:1], two, 32),
            lambda: ops.paged_attention_q4(q, cache, 0, t.long(), two, two, 32),
            lambda: ops.paged_attention_q4(q, cache, 0, t, two, two, 32, window=-1),
+           lambda: ops.paged_attention_q4(q, cache, 0, t, two, two, 32, window=(1 << 32) + 5),
+           lambda: ops.paged_attention_q4(q, cache, 0, t, two, two, 32, window=8, sinks=1 << 31),
+           lambda: ops.paged_attention_q4(q, cache, 1 << 32, t, two, two, 32),
+           lambda: ops.paged_attention_q4(q, cache, 0, t, two, two, (1 << 32) + 16),
+           lambda: ops.paged_attention_q4(torch.zeros(2 * 4 * 64 + 1, device=DEV)[1:].view(2, 4, 64), cache, 0, t, two,
+                                          two, 32),
+           lambda: ops.kv_read_q4(cache, m, k=torch.zeros(1, 2, 64, device=DEV).expand(3, 2, 64),
+                                  v=torch.zeros(3, 2, 64, device=DEV)),
+           lambda: ops.kv_write_q4(cache, rows, rows, m, layer=1 << 32),
            lambda: ops.paged_attention_q4(q, cache, 0, t, two, two, 32, rows_per_stream=3),
            lambda: ops.paged_attention_q4(q[:, :3], cache, 0, t, two, two, 32),
            lambda: ops.paged_attention_q4(q, cache, 0, t, two, two, 32, out=torch.empty(2, 255, device=DEV)),
@@ -542,6 +551,58 @@ def test_graph_streams_and_repeats(fmt):
     torch.cuda.synchronize()
     for i, o in enumerate(outs):
         assert torch.equal(o, want[i % 3])
+
+
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
+def test_garbage_queries_of_padded_rows(fmt):
+    """Rows without keys whose q holds NaN and infinity, among rows that have keys."""
+    H, D, S = 2, 128, 40
+    pool, vals = _pool(fmt, 4, 1, H, D, 5)
+    table = torch.arange(4, dtype=torch.int32).view(1, 4)
+    q = torch.randn(S, 4, D, generator=_gen(6))
+    q[:S // 2:2], q[1:S // 2:2] = float("nan"), float("inf")
+    ctx = torch.arange(S, dtype=torch.int32) - S // 2 + 1
+    ctx[:S // 2] = 0
+    slots = torch.zeros(S, dtype=torch.int32, device=DEV)
+    for s in (1, S):
+        out = _attend(fmt, q.to(DEV), pool, 0, table.to(DEV), slots, ctx.to(DEV), 64, rows_per_stream=s)
+        out = out.double().cpu().numpy()
+        assert not out[:S // 2].any()
+        for r in range(S // 2, S):
+            kv = vals[:, 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
+            want = O.attention(q[r].numpy(), kv[0], kv[1], int(ctx[r]))
+            assert (np.abs(out[r] - want) <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[r].numpy(), kv, True)).all()
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first calls are captured: the graph replays what eager calls give."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from test_stateful_b200 import ops
+cache = torch.zeros(8, 1, 2, 2, 9 * 64, dtype=torch.uint8, device="cuda")
+k = torch.randn(100, 2, 64, device="cuda"); m = torch.arange(100, dtype=torch.int32, device="cuda")
+q = torch.randn(100, 4, 64, device="cuda"); t = torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8)
+z = torch.zeros(100, dtype=torch.int32, device="cuda"); c = m + 1
+def step(s):
+    ops.kv_write_q4(cache, k, -k, m)
+    return ops.kv_read_q4(cache, m)[0], ops.paged_attention_q4(q, cache, 0, t, z, c, 128, 30, 2, rows_per_stream=s)
+torch.cuda.synchronize()
+s = torch.cuda.Stream()
+with torch.cuda.stream(s):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        a = step(1) + step(100)
+    g.replay()
+    s.synchronize()
+for x, y in zip(a, step(1) + step(100)):
+    assert torch.equal(x, y)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
