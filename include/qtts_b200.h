@@ -216,7 +216,8 @@ int qtts_paged_attention_noalloc(const void* q, int R, int num_heads, int kv_hea
  *   zero = fp16(min), scale = fp16((max - min) * fp32(1/15)) (fp32 steps), values saturated to
  *   +-65504 first; code = nearest integer to fp32(x - zero) / scale (exact quotient, ties to
  *   even), clamped to [0, 15], 0 where scale = 0;  value = code * scale + zero.
- * A NaN makes its group read back as NaN.
+ * A NaN makes its group read back as NaN.  Read as fp16, values past 65504 (a group that spans
+ * nearly all of fp16 can have some, up to 65600) are 65504.
  * Layout: [num_blocks][num_layers][2][kv_heads] chunks of QTTS_Q4_CHUNK_BYTES(head_dim) bytes, a
  * chunk = 16 tokens: 16 rows of head_dim / 2 bytes of codes, whose 32-bit words alternate between
  * the row's NG = head_dim / 64 groups (word NG * i + w = channels 64 w + 8 i .. + 7, the first in the

@@ -6,16 +6,19 @@
 //     P           = 2^(S - m)  one thread per row; fp16 to shared memory, two buffers
 //     O[128][D]  += P V        TMEM
 // Warps 0-3 are the softmax, warps 4-7 bring K and 8-11 V (one block a warp: cp.async for fp16; 4 bits
-// are turned into fp16 on the way through registers, fma(code, scale, zero) rounded once), warp 12 issues
-// the products, S one tile ahead of P V.  K and V tiles are panels of 64 channels, 128-byte rows with
+// are turned into fp16 on the way through registers, fma(code, scale, zero) rounded once and kept
+// finite as kv_read_q4 does), warp 12 issues the products, S one tile ahead of P V.  K and V tiles are panels of 64 channels, 128-byte rows with
 // the 128-byte swizzle; V is read in place as an MN-major operand.
 //
 // q enters as fp16 after a scaling by a power of two that brings the row's largest channel to
-// [2^11, 2^12): 2^-12 of each channel, as P's 2^-12 of each probability, a quarter of what the bf16
-// output rounds off; 4-bit values round to fp16 the same way.  Sums, maxima and O are fp32.
+// [2^11, 2^12): 2^-11 of each channel, as P's 2^-11 of each probability, an eighth of the 2^-8 that the
+// bf16 output rounds off; 4-bit values round to fp16 the same way.  Sums, maxima and O are fp32.
 //
-// Bound by: 128 x 64 exponentials a tile (512 cycles at 16 a cycle and SM) next to 512 cycles of
-// products at D = 128.  Every wait is bounded.
+// Bound by, a tile: 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the softmax does
+// around them, next to some 750 cycles of products at D = 128 (57 an instruction of N = 64, 75 of N = 128);
+// a launch adds some 7 us before its first products and after its last.  16 heads over 8, D = 128, B200: 8 x
+// 128 rows, 4 bits 16.6 us (227 TFLOP/s); 2 x 500 rows under a window of 256, fp16 19.6 us (110 TFLOP/s).
+// Every wait is bounded.
 #pragma once
 
 #include "attn_window.cuh"
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             // nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as fp16 pairs, times scale plus zero
             auto values = [&](uint32_t x, __half2 scale, __half2 zero) {
                 const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
-                              k64 = __floats2half2_rn(-64.f, -64.f);
+                              k64 = __floats2half2_rn(-64.f, -64.f), k65504 = __floats2half2_rn(65504.f, 65504.f);
                 uint4 u;
                 uint32_t* o = &u.x;
 #pragma unroll
@@ -391,7 +394,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     const uint32_t a = (y & 0x000f000fu) | 0x64006400u, b = (y & 0x00f000f0u) | 0x64006400u;
                     const __half2 ca = __hsub2(*reinterpret_cast<const __half2*>(&a), k1024);
                     const __half2 cb = __hfma2(*reinterpret_cast<const __half2*>(&b), k16, k64);
-                    const __half2 va = __hfma2(ca, scale, zero), vb = __hfma2(cb, scale, zero);
+                    const __half2 va = __hmin2_nan(__hfma2(ca, scale, zero), k65504),
+                                  vb = __hmin2_nan(__hfma2(cb, scale, zero), k65504);
                     o[2 * h] = *reinterpret_cast<const uint32_t*>(&va);
                     o[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&vb);
                 }

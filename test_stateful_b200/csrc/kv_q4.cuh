@@ -7,7 +7,8 @@
 //   code  = the integer in [0, 15] nearest to fl(x - zero) / scale, ties to even (0 when scale = 0)
 //   value = code * scale + zero
 // fl() is fp32 rounding; the quotient is taken exactly, so that the codes do not depend on how a
-// division rounds.  A NaN makes its group read back as NaN (zero = NaN, scale = 0, codes 0).
+// division rounds.  A NaN makes its group read back as NaN (zero = NaN, scale = 0, codes 0).  A group that
+// spans nearly all of fp16 can have values past 65504 (up to 65600, as scale was rounded): in fp16 they are 65504.
 //
 // Pool: [num_blocks][layers][2][kv_heads] chunks of 16 tokens.  A chunk is 16 rows of
 // head_dim / 2 bytes of codes, then head_dim / 64 arrays of 16 (scale, zero) fp16 pairs.  A row's
@@ -307,14 +308,16 @@ __global__ void __launch_bounds__(kQ4Threads) kv_read_q4_kernel(const Q4IoParams
                 // scale + zero is then one rounding of the exact value
                 const __half2 scale = __low2half2(prm[w]), zero = __high2half2(prm[w]);
                 const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
-                              k64 = __floats2half2_rn(-64.f, -64.f);
+                              k64 = __floats2half2_rn(-64.f, -64.f), k65504 = __floats2half2_rn(65504.f, 65504.f);
                 uint32_t v[4];  // channels (0, 4), (1, 5), (2, 6), (3, 7)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t u = wd >> (8 * h);
                     const uint32_t a = (u & 0x000f000fu) | 0x64006400u, b = (u & 0x00f000f0u) | 0x64006400u;
-                    const __half2 va = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&a), k1024), scale, zero);
-                    const __half2 vb = __hfma2(__hfma2(*reinterpret_cast<const __half2*>(&b), k16, k64), scale, zero);
+                    const __half2 ca = __hsub2(*reinterpret_cast<const __half2*>(&a), k1024);
+                    const __half2 cb = __hfma2(*reinterpret_cast<const __half2*>(&b), k16, k64);
+                    const __half2 va = __hmin2_nan(__hfma2(ca, scale, zero), k65504);
+                    const __half2 vb = __hmin2_nan(__hfma2(cb, scale, zero), k65504);
                     v[2 * h] = *reinterpret_cast<const uint32_t*>(&va);
                     v[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&vb);
                 }

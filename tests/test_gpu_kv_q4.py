@@ -120,6 +120,45 @@ def test_write_special_groups():
         _close_values(rv, vals[:, :, 1], torch.float32)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_groups_across_all_of_fp16_stay_finite(D):
+    """(65504 + 65504) / 15 rounds up to a scale of 8736, and 15 of it on -65504 is 65536: 65504 in fp16, read back,
+    gathered, and in either form of attention (half a step of 2^-11, which chunk tolerances count for a 4-bit value)."""
+    n = 80
+    k = torch.randn(n, 1, 1, D, generator=_gen(31))
+    k[:, :, :, 0], k[:, :, :, 1] = 65504, -65504
+    k[3, 0, 0, 2] = float("inf")
+    cache, m = _new_cache(5, 1, 1, D), torch.arange(n, dtype=torch.int32)
+    ops.kv_write_q4(cache, k.to(DEV), k.to(DEV), m.to(DEV))
+    want, vals = _expect(cache.shape, k, k, m.tolist(), 0)
+    _same_bytes(cache.cpu().numpy(), want, D)
+    assert vals.max() == 65536
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        rk, _ = ops.kv_read_q4(cache, m.to(DEV), dtype=dtype)
+        _close_values(rk, np.minimum(vals[:, :, 0], 65504) if dtype == torch.float16 else vals[:, :, 0], dtype)
+    flat = ops.kv_gather_q4(cache, torch.arange(5, dtype=torch.int32, device=DEV), n)
+    assert torch.isfinite(flat).all()
+    # queries small enough for scores of order one (0: every key counts the same)
+    S, kv = 64, vals[:, 0].transpose(1, 2, 0, 3)
+    table, ctx = torch.arange(5, dtype=torch.int32).view(1, 5), torch.arange(n - S, n, dtype=torch.int32) + 1
+    for qscale in (0.0, 1e-6):
+        q = torch.randn(S, 2, D, generator=_gen(32)) * qscale
+        for s in (1, S):
+            out = ops.paged_attention_q4(q.to(DEV), cache, 0, table.to(DEV), torch.zeros(S, dtype=torch.int32, device=DEV),
+                                         ctx.to(DEV), n, rows_per_stream=s).double().cpu().numpy()
+            for r in range(S):
+                w = O.attention(q[r].numpy(), kv[0], kv[1], int(ctx[r]))
+                tol = _tolerance("q4", q[r].numpy(), kv, s > 1)
+                assert (np.abs(out[r] - w) <= 2.0 ** -8 * np.abs(w) + tol).all(), (qscale, s, r)
+
+
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
+def test_queries_of_zero(fmt):
+    """Every visible key counts the same, hidden ones nothing, in either form."""
+    for S in (1, 90):
+        _run_case(fmt, 4, 2, 128, [100, 95], S, 40, 3, qscale=0.0)
+
+
 def test_write_many_random_borders():
     """Values drawn next to code borders, where a rounded quotient would decide wrongly."""
     g = _gen(9)
@@ -415,7 +454,7 @@ def test_both_chunk_forms(form):
 
     env = dict(os.environ, QTTS_WINDOW_TILES=form)
     r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k",
-                        "chunk or reach", os.path.abspath(__file__)], env=env, capture_output=True, text=True,
+                        "chunk or reach or finite or zero or garbage or bad or repeats", os.path.abspath(__file__)], env=env, capture_output=True, text=True,
                        timeout=900)
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
 
