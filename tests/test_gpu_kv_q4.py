@@ -593,6 +593,59 @@ def test_graph_streams_and_repeats(fmt):
 
 
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
+def test_chunks_with_bad_ids_captured_and_at_once(fmt):
+    """Eight chunks of 64 rows (128-row tiles): a slot and a block id outside their ranges, then captured, replayed
+    on new data, and two launches on two streams at once."""
+    H, D, S, n = 8, 64, 64, 8
+    pool, vals = _pool(fmt, 64, 1, H, D, 15)
+    table = torch.randperm(64, generator=_gen(16)).to(torch.int32).view(n, 8)
+    table[3, 1], table[4, 2] = 64, -7
+    q = torch.randn(n * S, 16, D, generator=_gen(17))
+    slots = torch.arange(n).repeat_interleave(S).to(torch.int32)
+    slots[5 * S:6 * S], slots[6 * S:7 * S] = -1, n
+    ctx = (torch.arange(S) + 40).repeat(n).to(torch.int32)
+    args = (pool, 0, table.to(DEV), slots.to(DEV), ctx.to(DEV), 128)
+    qd = q.to(DEV)
+    _lib.device_error()
+    out = _attend(fmt, qd, *args, window=50, sinks=3, rows_per_stream=S)
+    got = out.double().cpu().numpy()
+    assert _lib.device_error() == 8
+    assert not got[5 * S:7 * S].any()
+    for b in (0, 3, 4, 7):
+        ids = table[b].long()
+        kv = vals[ids.clamp(0, 63), 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
+        there = ((ids >= 0) & (ids < 64)).repeat_interleave(16).numpy()
+        for t in (0, 1, 20, S - 1):
+            r, c = b * S + t, int(ctx[t])
+            see = O.visible(c, 128, 50, 3) & there
+            want = O.attention(q[r].numpy(), kv[0][:, see], kv[1][:, see], int(see.sum()))
+            assert (np.abs(got[r] - want) <= 2.0 ** -8 * np.abs(want) + _tolerance(fmt, q[r].numpy(), kv, True)).all()
+    kw = dict(window=50, sinks=3, rows_per_stream=S)
+    other = torch.randn(n * S, 16, D, generator=_gen(18)).to(DEV)
+    want = [out.clone(), _attend(fmt, other, *args, **kw)]
+    torch.cuda.synchronize()
+    s, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            res = _attend(fmt, qd, *args, **kw)
+        for data, w in ((other.clone(), want[1]), (q.to(DEV), want[0])):
+            qd.copy_(data)
+            graph.replay()
+            s.synchronize()
+            assert torch.equal(res, w)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(s):
+            a = _attend(fmt, qd, *args, **kw)
+        with torch.cuda.stream(s2):
+            b = _attend(fmt, other, *args, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    assert _lib.device_error() == 8
+
+
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
 def test_garbage_queries_of_padded_rows(fmt):
     """Rows without keys whose q holds NaN and infinity, among rows that have keys."""
     H, D, S = 2, 128, 40
