@@ -28,6 +28,11 @@
 // The channel order of the contractions is the one in which a lane's words arrive: lane (g, t) takes
 // of K tokens g and g + 8 the channels 64 w + 16 t .. + 15, of V tokens 2 t, 2 t + 1, 2 t + 8,
 // 2 t + 9 the channels 64 w + 8 g .. + 7.
+//
+// Bound by (16 heads over 8, D = 128, B200): fp16 by HBM, 64 x 4096 keys 172 us (6.25 TB/s); 4 bits by the
+// integer pipe next to HBM, the same keys 64 us (4.7 TB/s).  A decode step of one wave by latencies (block
+// ids, first copies, the longest row): 64 streams of 260 .. 780 keys at 4 bits 17 us, under a window of 72 +
+// 4 over fp16 12 us.
 #pragma once
 
 #include <type_traits>
