@@ -665,7 +665,9 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int sl = (2 * t + e) % SL;
-        if (ctx[e] == 0) l[e] = 0.f;  // a row without keys in a tile of rows that have some
+        // a row without keys in a tile of rows that have some: whole blocks scored its q unmasked, so its sum may
+        // be anything and its maximum infinite (inf - inf would make the folds' factors NaN)
+        if (ctx[e] == 0) l[e] = 0.f, m[e] = -INFINITY;
 #pragma unroll
         for (int x = SL / 2; x < 32; x <<= 1) {
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);

@@ -1,0 +1,47 @@
+"""Corners of the 4-bit KV cache and of windowed paged attention, against the float64 oracle.
+
+Tolerances are those of ``test_gpu_kv_q4`` (derived there) unless a test derives its own."""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from oracle import kv_q4 as O  # noqa: E402
+from test_stateful_b200 import _lib  # noqa: E402
+from tests.test_gpu_kv_q4 import DEV, _attend, _gen, _tolerance  # noqa: E402
+
+
+# ------------------------------------------------------------------------------ rows without keys
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
+@pytest.mark.parametrize("S,pad,last", [(38, 5, 100), (38, 5, 1500), (90, 27, 200), (90, 27, 520)])
+@pytest.mark.parametrize("Hq,H,D", [(4, 2, 128), (8, 2, 64)])
+def test_padded_rows_beside_whole_blocks(fmt, S, pad, last, Hq, H, D):
+    """The last rows of a chunk are padding (context 0) whose q holds what memory held: finite numbers whose scores
+    overflow, one infinite channel, NaN.  The other rows of their tile see whole blocks, so that no mask is
+    applied there; keys of the long ones are shared by CTAs of a cluster."""
+    nb = -(-last // 16)
+    # keys of one sign, so that a huge q's scores overflow to +infinity over 4 bits too (zeros near 0)
+    x = (torch.randn(nb, 1, 2, H, 16, D, generator=_gen(5)).abs() * 4).half()
+    raw = x.numpy() if fmt == "fp16" else O.pack(*O.quantise(x.float().numpy()))
+    pool, vals = torch.from_numpy(raw).to(DEV), x.double().numpy() if fmt == "fp16" else O.unpack(raw)
+    table = torch.arange(nb, dtype=torch.int32).view(1, nb)
+    q = torch.randn(S, Hq, D, generator=_gen(6)) / 4
+    real = S - pad
+    ctx = torch.zeros(S, dtype=torch.int32)
+    ctx[:real] = torch.arange(last - real + 1, last + 1)
+    fills = [lambda x: x[:, 3].fill_(3e38), lambda x: x.fill_(3e38), lambda x: x[:, 3].fill_(float("inf")),
+             lambda x: x.mul_(1e38), lambda x: x.fill_(float("nan")), lambda x: x.fill_(float("inf"))]
+    for r in range(real, S):
+        fills[(r - real) % len(fills)](q[r])
+    lo = torch.full((S, Hq * D), 9.0, device=DEV, dtype=torch.bfloat16)
+    out = _attend(fmt, q.to(DEV), pool, 0, table.to(DEV), torch.zeros(S, dtype=torch.int32, device=DEV), ctx.to(DEV), last,
+                  rows_per_stream=S, out_lo=lo)
+    assert _lib.device_error() == 0
+    assert not out[real:].any() and not lo[real:].any()
+    got = (out.double() + lo.double()).cpu().numpy()
+    kv = vals[:, 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
+    for r in range(0, real, 7):
+        want = O.attention(q[r].numpy(), kv[0], kv[1], int(ctx[r]))
+        assert np.abs(got[r] - want).max() <= _tolerance(fmt, q[r].numpy(), kv, True), r
