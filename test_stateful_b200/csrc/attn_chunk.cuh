@@ -530,7 +530,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     }
 
     // ---------------------------------------------------------------------- out
-    if (ctx == 0) l = 0.f;  // a row without keys in a tile of rows that have some
+    // a row without keys in a tile of rows that have some: whole tiles scored its q unmasked, so its sum may be
+    // anything and its maximum infinite (inf - inf would make the fold's factor NaN)
+    if (ctx == 0) l = 0.f, m = -INFINITY;
     float* part = reinterpret_cast<float*>(smem + L::RING);
     auto out_at = [&](int row, int d) { return head_row(row) * D + d; };
     __syncwarp();

@@ -2,6 +2,10 @@
 
 Tolerances are those of ``test_gpu_kv_q4`` (derived there) unless a test derives its own."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -11,6 +15,8 @@ pytestmark = pytest.mark.gpu
 from oracle import kv_q4 as O  # noqa: E402
 from test_stateful_b200 import _lib  # noqa: E402
 from tests.test_gpu_kv_q4 import DEV, _attend, _gen, _tolerance  # noqa: E402
+
+FORCED = os.environ.get("QTTS_WINDOW_TILES")
 
 
 # ------------------------------------------------------------------------------ rows without keys
@@ -45,3 +51,14 @@ def test_padded_rows_beside_whole_blocks(fmt, S, pad, last, Hq, H, D):
     for r in range(0, real, 7):
         want = O.attention(q[r].numpy(), kv[0], kv[1], int(ctx[r]))
         assert np.abs(got[r] - want).max() <= _tolerance(fmt, q[r].numpy(), kv, True), r
+
+
+@pytest.mark.skipif(FORCED is not None, reason="already a forced run")
+@pytest.mark.parametrize("form", ["0", "1"])
+def test_both_chunk_forms(form):
+    """The chunk cases of this file through 8-row and 128-row tiles (QTTS_WINDOW_TILES is read once per process)."""
+    env = dict(os.environ, QTTS_WINDOW_TILES=form)
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k",
+                        "padded", os.path.abspath(__file__)], env=env, capture_output=True, text=True, timeout=900,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
