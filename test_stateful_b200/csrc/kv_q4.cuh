@@ -217,6 +217,14 @@ __global__ void __launch_bounds__(kQ4Threads) kv_write_q4_kernel(const Q4IoParam
         // of zeros of both signs, +0
         const float lo = __fadd_rn(fminf(fmaxf(range.x, -65504.f), 65504.f), 0.f);
         const float hi = fminf(fmaxf(range.y, -65504.f), 65504.f);
+        // The values saturate as the range does: where fp16(lo) rounds up near 65504, a larger value is not 15 steps
+        // away.  16-bit types step so far there that it always is, and below -65504 the code is 0 either way.
+        if constexpr (sizeof(T) == 4) {
+            if (range.y > 65504.f) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) x[w][c] = fminf(x[w][c], 65504.f);
+            }
+        }
         const __half zero_h = nan ? __ushort_as_half(0x7fff) : __float2half_rn(lo);
         const __half scale_h = nan ? __float2half_rn(0.f)
                                    : __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));

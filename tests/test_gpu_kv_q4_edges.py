@@ -13,8 +13,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from oracle import kv_q4 as O  # noqa: E402
-from test_stateful_b200 import _lib  # noqa: E402
-from tests.test_gpu_kv_q4 import DEV, _attend, _gen, _tolerance  # noqa: E402
+from test_stateful_b200 import _lib, ops  # noqa: E402
+from tests.test_gpu_kv_q4 import DEV, _attend, _expect, _gen, _new_cache, _same_bytes, _tolerance  # noqa: E402
 
 FORCED = os.environ.get("QTTS_WINDOW_TILES")
 
@@ -51,6 +51,28 @@ def test_padded_rows_beside_whole_blocks(fmt, S, pad, last, Hq, H, D):
     for r in range(0, real, 7):
         want = O.attention(q[r].numpy(), kv[0], kv[1], int(ctx[r]))
         assert np.abs(got[r] - want).max() <= _tolerance(fmt, q[r].numpy(), kv, True), r
+
+
+# ------------------------------------------------------------------------------ the cache
+def test_write_groups_that_saturate_near_the_top():
+    """fp32 values past 65504 are 65504 before they are coded, also where the group's zero is near 65504 itself (fp16(min)
+    may round up, so that (65504 - zero) / scale is far from 15)."""
+    g = _gen(41)
+    n = 400
+    lo = 65504 - torch.rand(n, 1, 1, 1, generator=g) * 10.0 ** (torch.rand(n, 1, 1, 1, generator=g) * 3.5 - 0.5)
+    x = lo + (65504 - lo) * torch.rand(n, 1, 1, 128, generator=g)
+    far = torch.rand(n, 1, 1, 128, generator=g) < 0.05
+    x[far] = 65504 + 10.0 ** (torch.rand(int(far.sum()), generator=g) * 30)
+    x[0], x[0, :, :, 7] = 65400.0, 1e6
+    x[1], x[1, :, :, 7] = 65495.0, 1e6
+    x[2], x[2, :, :, 7] = 65457.0, float("inf")
+    x[3], x[3, :, :, :] = 65504.0, 70000.0
+    assert (O.quantise(x[:2].numpy())[0][:, 0, 0, 0, 7] == [14, 0]).all()
+    m = torch.arange(n, dtype=torch.int32)
+    cache = _new_cache(n // 16, 1, 1, 128)
+    ops.kv_write_q4(cache, x.to(DEV), (-x).to(DEV), m.to(DEV))
+    want, _ = _expect(cache.shape, x, -x, m.tolist(), 0)
+    _same_bytes(cache.cpu().numpy(), want, 128)
 
 
 @pytest.mark.skipif(FORCED is not None, reason="already a forced run")
