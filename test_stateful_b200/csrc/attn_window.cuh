@@ -163,6 +163,11 @@ struct WinChunk {
 constexpr float kPScale = 1.2676506002282294e30f;  // 2^100
 constexpr float kPUnscale = 8589934592.f;          // 2^133 / 2^100
 
+// fp16 halves of a probability: it is taken relative to 2^-7 of the running maximum, which leaves it below 2^15 (the
+// maximum may lag by 2^8) and puts fp16's last step at 2^-31 of the maximum.  Relative to the maximum itself,
+// keys below 2^-25 of it would vanish from O but not from the sum: 32000 of them, 1e-3 of the output.
+constexpr float kPShift = 7.f;
+
 constexpr int kWinMaxSplits = 16;  // CTAs of a cluster
 
 // ld.shared::cluster that several of may be under way (no memory clobber): the data was published by
@@ -371,7 +376,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
 
     float o[MT][4];  // FMT q4: row tile 4 w + k holds channels 64 w + 8 g + 2 k (c 0, 1) and + 1 (c 2, 3)
     float zacc[NW][2], l[2] = {0.f, 0.f};
-    // running maximum of the two columns' slots, and what probabilities are relative to (0 until a key is seen)
+    // running maximum of the two columns' slots, and what probabilities are relative to (the maximum, or 2^-7 of it
+    // over fp16; 0 until a key is seen)
     float m[2] = {-INFINITY, -INFINITY}, mu[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -484,11 +490,12 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
                 if (!sees(i)) s[i] = -INFINITY;
         }
 
-        // softmax in the log2 domain; the running maximum moves only when a score passes it by
-        // 8, so that probabilities stay below 2^8
+        // softmax in the log2 domain; the running maximum moves only when a score passes it by 8, so that
+        // probabilities stay below 2^8 (fp16: 2^15)
+        constexpr float kShift = FMT == kWinF16 ? kPShift : 0.f;
         bool grow = false;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) grow |= fmaxf(s[e], s[2 + e]) > (m[e] == -INFINITY ? -INFINITY : 8.f);
+        for (int e = 0; e < 2; ++e) grow |= fmaxf(s[e], s[2 + e]) > (m[e] == -INFINITY ? -INFINITY : 8.f + kShift);
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -497,7 +504,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
                 for (int x = SL / 2; x < 32; x <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
                 mn = fmaxf(mn, m[e]);
                 const float corr = mn == -INFINITY ? 1.f : ex2_approx(m[e] - mn);
-                const float to = mn == -INFINITY ? 0.f : mn;
+                const float to = mn == -INFINITY ? 0.f : mn - kShift;
                 s[e] += mu[e] - to;
                 s[2 + e] += mu[e] - to;
                 m[e] = mn;

@@ -53,6 +53,42 @@ def test_padded_rows_beside_whole_blocks(fmt, S, pad, last, Hq, H, D):
         assert np.abs(got[r] - want).max() <= _tolerance(fmt, q[r].numpy(), kv, True), r
 
 
+# ------------------------------------------------------------------------------ small probabilities
+def _dominant(fmt, n, at, D, fall):
+    """A pool of one KV head and n keys, key ``at`` of value 0 scoring ``fall`` (nats) above all others for q = 8 e_0; the
+    others' values lie in [4, 12].  Returns pool, keys and values [2, 1, n, D]."""
+    nb = -(-n // 16)
+    x = torch.zeros(nb * 16, 2, D)
+    x[at, 0, 0] = fall * D ** 0.5 / 8
+    x[:, 1] = 4 + 8 * torch.rand(nb * 16, D, generator=_gen(at))
+    x[at, 1] = 0
+    x = x.view(nb, 16, 2, 1, D).permute(0, 2, 3, 1, 4).unsqueeze(1).contiguous().half()
+    raw = x.numpy() if fmt == "fp16" else O.pack(*O.quantise(x.float().numpy()))
+    vals = x.double().numpy() if fmt == "fp16" else O.unpack(raw)
+    return torch.from_numpy(raw).to(DEV), vals[:, 0].transpose(1, 2, 0, 3, 4).reshape(2, 1, -1, D)[:, :, :n]
+
+
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("at", [0, 17000, 32000])
+def test_many_small_probabilities_beside_a_dominant_key(fmt, D, at):
+    """32000 keys below 2^-25 of the largest probability are 1e-3 of the sum: they count in the output as they do there.
+    Tolerance: a probability's fp16 halves end at 2^-32 of the maximum (half of 2^-31), n of them; relative errors of
+    scores (27 in log2 units x 2^-22), ex2 (2^-22), probabilities (2^-16), sums and output (2^-17) below 2^-14."""
+    n, rows = 32001, 300  # more tiles than CTAs fit at once: keys are not split, a warp walks thousands of them
+    pool, kv = _dominant(fmt, n, at, D, 18.3)
+    q = torch.zeros(rows, 2, D)
+    q[:, :, 0] = 8
+    zero = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    lo = torch.empty(rows, 2 * D, device=DEV, dtype=torch.bfloat16)
+    out = _attend(fmt, q.to(DEV), pool, 0, torch.arange(pool.shape[0], dtype=torch.int32, device=DEV).view(1, -1), zero,
+                  zero + n, n, out_lo=lo)
+    got = (out.double() + lo.double()).cpu().numpy()
+    want = O.attention(q[0].numpy(), kv[0], kv[1], n)
+    assert want.min() > 1e-3
+    assert (np.abs(got - want) <= n * 2.0 ** -32 * 12 + 2.0 ** -14 * want).all()
+
+
 # ------------------------------------------------------------------------------ the cache
 def test_write_groups_that_saturate_near_the_top():
     """fp32 values past 65504 are 65504 before they are coded, also where the group's zero is near 65504 itself (fp16(min)
