@@ -3,7 +3,7 @@
 // One CTA takes 128 rows (row = query * group + head: the query heads of one KV head for consecutive
 // queries of a stream) through tiles of four 16-token blocks, only those that hold a key some row sees:
 //     S[128][64]  = Q K^T      TMEM, two buffers
-//     P           = 2^(S - m)  one thread per row; fp16 to shared memory, two buffers
+//     P           = 2^(S - m)  TMEM, two buffers: one thread per row writes it as fp16 pairs, high and low halves
 //     O[128][D]  += P V        TMEM
 // Warps 0-3 are the softmax, warps 4-7 bring K and 8-11 V (one block a warp: cp.async for fp16; 4 bits
 // are turned into fp16 on the way through registers, fma(code, scale, zero) rounded once and kept
@@ -11,13 +11,16 @@
 // the 128-byte swizzle; V is read in place as an MN-major operand.
 //
 // q enters as fp16 after a scaling by a power of two that brings the row's largest channel to
-// [2^11, 2^12): 2^-11 of each channel, as P's 2^-11 of each probability, an eighth of the 2^-8 that the
-// bf16 output rounds off; 4-bit values round to fp16 the same way.  Sums, maxima and O are fp32.
+// [2^11, 2^12), and P relative to 2^-7 of the running maximum, both as pairs of a high half and what it leaves: 22
+// bits, as the row kernel has, so that the form a call goes through is not seen in its output's low half.
+// (Single halves, 2^-11 of q, move a score by up to 2^-11 sum |q k| / sqrt(D): with loud channels more than
+// the bf16 output rounds off.)  4-bit values round to fp16.  Sums, maxima and O are fp32.
 //
-// Bound by, a tile: 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the softmax does
-// around them, next to some 750 cycles of products at D = 128 (57 an instruction of N = 64, 75 of N = 128);
-// a launch adds some 7 us before its first products and after its last.  16 heads over 8, D = 128, B200: 8 x
-// 128 rows, 4 bits 16.6 us (227 TFLOP/s); 2 x 500 rows under a window of 256, fp16 19.6 us (110 TFLOP/s).
+// Bound by, a tile: 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the softmax does around
+// them, next to some 1600 cycles of products at D = 128 (57 an instruction of N = 64 for S, 88 of N = 128 for P V); a
+// launch adds some 7 us before its first products and after its last.  16 heads over 8, D = 128, B200: 8 x 128
+// rows, 4 bits 18.4 us (204 TFLOP/s; single halves: 16.7); 2 x 500 rows under a window of 256, fp16 21.1 us (102
+// TFLOP/s; 19.6).
 // Every wait is bounded.
 #pragma once
 
@@ -47,6 +50,17 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
     for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// 32 lanes x 32 bits, 16 consecutive columns; tmem_st_wait() after the last of several
+__device__ __forceinline__ void tmem_st16_now(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -61,15 +75,16 @@ struct ChunkLayout {
     static constexpr int RAW = FMT == kWinQ4 ? 4 : 0; // tiles of codes on their way (cp.async), before they are turned into fp16
     static constexpr int PANEL = 64 * 128;            // 64 keys x 64 channels
     static constexpr int STAGE = 2 * NW * PANEL;      // K panels, V panels
-    static constexpr int Q = 0;                       // NW panels of 128 rows
-    static constexpr int RING = Q + NW * 128 * 128;
-    static constexpr int P = RING + ST * STAGE;
-    static constexpr int CODES = P + 2 * 128 * 128;   // [K, V][warp][RAW] chunks
+    static constexpr int QHALF = NW * 128 * 128;      // NW panels of 128 rows
+    static constexpr int Q = 0;                       // high halves, low halves
+    static constexpr int RING = Q + 2 * QHALF;
+    static constexpr int CODES = RING + ST * STAGE;   // [K, V][warp][RAW] chunks
     static constexpr int SMEM = CODES + 4 * RAW * 2 * WinChunk<FMT, D>::BYTES + 1024;
     static constexpr int PART = D + 4;                // floats per row of a partial output (no bank met twice)
     static constexpr int ROWB = 2 * D + 16;           // bytes per row of a bf16 output
-    static_assert(128 * PART * 4 <= ST * STAGE + 2 * 128 * 128 && 2 * 128 * ROWB <= ST * STAGE + 2 * 128 * 128,
-                  "outputs replace ring and P");
+    static_assert(128 * PART * 4 <= ST * STAGE && 2 * 128 * ROWB <= ST * STAGE, "outputs replace the ring");
+    // TMEM columns: S (two buffers of 64), O, P (two buffers of 32 for the high halves of 64 keys, 32 for the low)
+    static constexpr uint32_t TS = 0, TO = 128, TP = 256, TCOLS = 512;
     static_assert(SMEM + 4096 <= 227 * 1024, "tile exceeds shared memory");
 };
 
@@ -149,7 +164,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             fence_mbar_init();
         }
         __syncwarp();
-        tmem_alloc(&s_tmem, 256);
+        tmem_alloc(&s_tmem, L::TCOLS);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -270,15 +285,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 top = __reduce_max_sync(RPI == 1 ? 0xffffffffu : 0xffffu << (lane & 16), top);
                 const int ex = max((int)(top >> 23), 12);
                 const float up = __uint_as_float((uint32_t)(265 - ex) << 23);
-                uint2 h = make_uint2(pack_h2(u.x * up, u.y * up), pack_h2(u.z * up, u.w * up));
-                if constexpr (FMT == kWinQ4) {
-                    // the channel order in which nibbles come apart (below): 0 4 1 5 2 6 3 7 of each eight.
-                    // An even lane holds 0 1 2 3 and makes 0 4 1 5, the odd one beside it 4 5 6 7 and 2 6 3 7
-                    const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? h.x : h.y, 1);
-                    h = lane & 1 ? make_uint2(prmt(other, h.y, 0x5410), prmt(other, h.y, 0x7632))
-                                 : make_uint2(prmt(h.x, other, 0x5410), prmt(h.x, other, 0x7632));
+                uint2 h[2];  // high and low halves
+                split_h2(u.x * up, u.y * up, h[0].x, h[1].x);
+                split_h2(u.z * up, u.w * up, h[0].y, h[1].y);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint2& x = h[half];
+                    if constexpr (FMT == kWinQ4) {
+                        // the channel order in which nibbles come apart (below): 0 4 1 5 2 6 3 7 of each eight.
+                        // An even lane holds 0 1 2 3 and makes 0 4 1 5, the odd one beside it 4 5 6 7 and 2 6 3 7
+                        const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x.x : x.y, 1);
+                        x = lane & 1 ? make_uint2(prmt(other, x.y, 0x5410), prmt(other, x.y, 0x7632))
+                                     : make_uint2(prmt(x.x, other, 0x5410), prmt(x.x, other, 0x7632));
+                    }
+                    *reinterpret_cast<uint2*>(smem + L::Q + half * L::QHALF + (c >> 4) * 16384 +
+                                              sw128_off(row, (c & 15) * 4)) = x;
                 }
-                *reinterpret_cast<uint2*>(smem + L::Q + (c >> 4) * 16384 + sw128_off(row, (c & 15) * 4)) = h;
                 if (c == 0) s_sf[row] = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
             }
 #pragma unroll
@@ -302,7 +324,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             if (!ok) break;
             tc_fence_after();
             float v[64];
-            tmem_ld64(lanes + (i & 1) * 64, v);
+            tmem_ld64(lanes + L::TS + (i & 1) * 64, v);
             const uint32_t here = *reinterpret_cast<const uint32_t*>(s_here[st]);
             const bool whole = here == 0x01010101u && t0 + i >= whole0 && t0 + i < whole1;
             if (!whole) {
@@ -336,12 +358,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             // sf > 0; -inf stays
             const float top = sf * fmaxf(fmaxf(fmaxf(t8[0], t8[1]), fmaxf(t8[2], t8[3])),
                                          fmaxf(fmaxf(t8[4], t8[5]), fmaxf(t8[6], t8[7])));
-            // the running maximum moves only when a score passes it by 8: P < 2^8
+            // the running maximum moves only when a score passes it by 8; P, relative to 2^-7 of it, stays below 2^15
             if (__any_sync(0xffffffffu, top > (m == -INFINITY ? -INFINITY : m + 8.f))) {
                 const float mn = fmaxf(m, top);
                 const float corr = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
                 m = mn;
-                mu = mn == -INFINITY ? 0.f : mn;
+                mu = mn == -INFINITY ? 0.f : mn - kPShift;
                 l *= corr;
                 if (i > 0) {  // O holds P V of tiles 0 .. i - 1 once the last is done
                     ok = mbar_wait(&pv_done[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u, DEV_ERR_ATTN_WAIT);
@@ -351,28 +373,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
 #pragma unroll 1
                     for (int c = 0; c < D; c += 16) {
                         float x[16];
-                        tmem_ld16(lanes + 128 + c, x);
+                        tmem_ld16(lanes + L::TO + c, x);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) x[k] *= corr;
-                        tmem_st16(lanes + 128 + c, x);
+                        tmem_st16(lanes + L::TO + c, x);
                     }
                 }
             }
             float s4[4] = {0.f, 0.f, 0.f, 0.f};
-            uint8_t* pr = smem + L::P + (i & 1) * 16384;
+            const uint32_t to_p = lanes + L::TP + (i & 1) * 64;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                uint32_t u[4];
+            for (int c = 0; c < 2; ++c) {  // 32 keys: 16 columns of two each
+                uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float a = ex2_approx(fmaf(v[8 * c + 2 * k], sf, -mu)), b = ex2_approx(fmaf(v[8 * c + 2 * k + 1], sf, -mu));
-                    s4[k] += a + b;
-                    u[k] = pack_h2(a, b);
+                for (int k = 0; k < 16; ++k) {
+                    const float a = ex2_approx(fmaf(v[32 * c + 2 * k], sf, -mu)), b = ex2_approx(fmaf(v[32 * c + 2 * k + 1], sf, -mu));
+                    s4[k & 3] += a + b;
+                    split_h2(a, b, hi[k], lo[k]);
                 }
-                *reinterpret_cast<uint4*>(pr + sw128_off(r, 8 * c)) = make_uint4(u[0], u[1], u[2], u[3]);
+                tmem_st16_now(to_p + 16 * c, hi);
+                tmem_st16_now(to_p + 32 + 16 * c, lo);
             }
+            tmem_st_wait();
             l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            fence_proxy_async_smem();
             tc_fence_before();
             mbar_arrive(&p_full[i & 1]);
         }
@@ -486,18 +509,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         const uint32_t idesc_s = make_idesc_f16(128, 64), idesc_o = make_idesc_f16(128, D) | (1u << 16);  // V is MN-major
         // descriptors of the buffers' starts; a step's is an addition to the address field (16-byte units)
         const uint64_t q_desc = make_sw128_desc(smem_u32(smem + L::Q)), k_desc = make_sw128_desc(smem_u32(smem + L::RING)),
-                       p_desc = make_sw128_desc(smem_u32(smem + L::P)),
                        v_desc = make_sw128_mn_desc(smem_u32(smem + L::RING + NW * L::PANEL), L::PANEL);
         auto issue_s = [&](int i) {
             if (!mbar_wait(&k_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT)) return false;
             tc_fence_after();
             const uint64_t kd = k_desc + (uint32_t)((i % ST) * (L::STAGE >> 4));
-            const uint32_t d = tmem + (i & 1) * 64;
+            const uint32_t d = tmem + L::TS + (i & 1) * 64;
             if (lead) {
 #pragma unroll
-                for (int kk = 0; kk < 4 * NW; ++kk)
-                    umma_bf16(d, q_desc + ((kk >> 2) * (16384 >> 4) + 2 * (kk & 3)),
-                              kd + ((kk >> 2) * (L::PANEL >> 4) + 2 * (kk & 3)), idesc_s, kk ? 1u : 0u);
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int kk = 0; kk < 4 * NW; ++kk)
+                        umma_bf16(d, q_desc + (half * (L::QHALF >> 4) + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3)),
+                                  kd + ((kk >> 2) * (L::PANEL >> 4) + 2 * (kk & 3)), idesc_s, (half | kk) ? 1u : 0u);
                 umma_commit(&s_full[i & 1]);
             }
             return true;
@@ -510,11 +534,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t pd = p_desc + (uint32_t)((i & 1) * (16384 >> 4)), vd = v_desc + (uint32_t)((i % ST) * (L::STAGE >> 4));
+            const uint64_t vd = v_desc + (uint32_t)((i % ST) * (L::STAGE >> 4));
+            const uint32_t pt0 = tmem + L::TP + (i & 1) * 64;
             if (lead) {
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    umma_bf16(tmem + 128u, pd + 2 * kk, vd + kk * (2048 >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_ts_f16(tmem + L::TO, pt0 + half * 32 + kk * 8, vd + kk * (2048 >> 4), idesc_o,
+                                    (i > 0 || half > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(&empty[i % ST]);
                 umma_commit(&pv_done[i & 1]);
             }
@@ -537,7 +565,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     auto out_at = [&](int row, int d) { return head_row(row) * D + d; };
     __syncwarp();
     if (warp < 4) {
-        const uint32_t lanes = tmem + ((uint32_t)warp << 21) + 128;
+        const uint32_t lanes = tmem + ((uint32_t)warp << 21) + L::TO;
         const bool sum = ok && nt > 0 && l != 0.f;  // else zeros (NaN counts as a sum)
         const float inv = splits == 1 ? 1.f / l : 1.f;
         uint8_t* staged = smem + L::RING;  // [row][ROWB] bf16, then the low halves
@@ -580,7 +608,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 256);
+    if (warp == 12) tmem_dealloc(tmem, L::TCOLS);
     if (splits == 1) {
         // whole rows leave shared memory
         for (int k = threadIdx.x; k < rows * (D / 8); k += kChunkThreads) {

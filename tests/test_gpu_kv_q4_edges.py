@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 from oracle import kv_q4 as O  # noqa: E402
 from test_stateful_b200 import _lib, ops  # noqa: E402
-from tests.test_gpu_kv_q4 import DEV, _attend, _expect, _gen, _new_cache, _same_bytes, _tolerance  # noqa: E402
+from tests.test_gpu_kv_q4 import DEV, _attend, _expect, _gen, _new_cache, _pool, _same_bytes, _tolerance  # noqa: E402
 
 FORCED = os.environ.get("QTTS_WINDOW_TILES")
 
@@ -71,7 +71,8 @@ def _dominant(fmt, n, at, D, fall):
 @pytest.mark.parametrize("fmt", ["q4", "fp16"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("at", [0, 17000, 32000])
-def test_many_small_probabilities_beside_a_dominant_key(fmt, D, at):
+@pytest.mark.parametrize("S", [1, 300])
+def test_many_small_probabilities_beside_a_dominant_key(fmt, D, at, S):
     """32000 keys below 2^-25 of the largest probability are 1e-3 of the sum: they count in the output as they do there.
     Tolerance: a probability's fp16 halves end at 2^-32 of the maximum (half of 2^-31), n of them; relative errors of
     scores (27 in log2 units x 2^-22), ex2 (2^-22), probabilities (2^-16), sums and output (2^-17) below 2^-14."""
@@ -82,11 +83,44 @@ def test_many_small_probabilities_beside_a_dominant_key(fmt, D, at):
     zero = torch.zeros(rows, dtype=torch.int32, device=DEV)
     lo = torch.empty(rows, 2 * D, device=DEV, dtype=torch.bfloat16)
     out = _attend(fmt, q.to(DEV), pool, 0, torch.arange(pool.shape[0], dtype=torch.int32, device=DEV).view(1, -1), zero,
-                  zero + n, n, out_lo=lo)
+                  zero + n, n, rows_per_stream=S, out_lo=lo)
     got = (out.double() + lo.double()).cpu().numpy()
     want = O.attention(q[0].numpy(), kv[0], kv[1], n)
     assert want.min() > 1e-3
     assert (np.abs(got - want) <= n * 2.0 ** -32 * 12 + 2.0 ** -14 * want).all()
+
+
+# ------------------------------------------------------------------------------ precision of chunks
+def _chunk(fmt, S, past, Hq, H, D, qscale, seed=0):
+    """Out + out_lo, the oracle's and the values' root mean square of every ninth row of a chunk of S after ``past`` keys."""
+    n = S + past
+    nb = -(-n // 16)
+    pool, vals = _pool(fmt, nb, 1, H, D, seed + 11)
+    q = torch.randn(S, Hq, D, generator=_gen(seed + 12)) * qscale
+    zero = torch.zeros(S, dtype=torch.int32, device=DEV)
+    ctx = torch.arange(past + 1, n + 1, dtype=torch.int32)
+    lo = torch.empty(S, Hq * D, device=DEV, dtype=torch.bfloat16)
+    out = _attend(fmt, q.to(DEV), pool, 0, torch.arange(nb, dtype=torch.int32, device=DEV).view(1, nb), zero, ctx.to(DEV), n,
+                  rows_per_stream=S, out_lo=lo)
+    got = (out.double() + lo.double()).cpu().numpy()
+    kv = vals[:, 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
+    rows = range(0, S, 9)
+    want = np.stack([O.attention(q[r].numpy(), kv[0], kv[1], past + 1 + r) for r in rows])
+    return got[list(rows)], want, np.sqrt((kv[1] ** 2).mean())
+
+
+@pytest.mark.parametrize("fmt", ["fp16"])
+@pytest.mark.parametrize("Hq,H,D", [(4, 2, 128), (8, 2, 64)])
+@pytest.mark.parametrize("S,past,qscale", [(150, 3, 1.0), (150, 100, 4.0), (70, 900, 2.0)])
+def test_chunks_keep_sixteen_bits(fmt, Hq, H, D, S, past, qscale):
+    """Out + out_lo of a chunk, root mean square over a row, whichever form the call goes through.  The output's halves
+    leave 2^-17 of it, a probability's pair 2^-17 or less of it (its errors at random over the keys, and no more than
+    one key's); q is held to 2^-20 of its largest channel or better, below 2^-20 * 3 qscale |k| / sqrt(D) <= 2^-17 qscale
+    of a score, products and their fp32 sums less.  A probability moves by twice a score's error: together 2^-16 (1 +
+    qscale) of the values, which rounding at random stays well below."""
+    got, want, rms_v = _chunk(fmt, S, past, Hq, H, D, qscale)
+    err = np.sqrt(((got - want) ** 2).mean(-1))
+    assert err.max() <= 2.0 ** -16 * (1 + qscale) * rms_v, err.max() / rms_v
 
 
 # ------------------------------------------------------------------------------ the cache
@@ -117,6 +151,6 @@ def test_both_chunk_forms(form):
     """The chunk cases of this file through 8-row and 128-row tiles (QTTS_WINDOW_TILES is read once per process)."""
     env = dict(os.environ, QTTS_WINDOW_TILES=form)
     r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k",
-                        "padded", os.path.abspath(__file__)], env=env, capture_output=True, text=True, timeout=900,
+                        "padded or chunks or small", os.path.abspath(__file__)], env=env, capture_output=True, text=True, timeout=900,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
