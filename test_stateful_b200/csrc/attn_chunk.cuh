@@ -6,21 +6,23 @@
 //     P           = 2^(S - m)  TMEM, two buffers: one thread per row writes it as fp16 pairs, high and low halves
 //     O[128][D]  += P V        TMEM
 // Warps 0-3 are the softmax, warps 4-7 bring K and 8-11 V (one block a warp: cp.async for fp16; 4 bits
-// are turned into fp16 on the way through registers, fma(code, scale, zero) rounded once and kept
-// finite as kv_read_q4 does), warp 12 issues the products, S one tile ahead of P V.  K and V tiles are panels of 64 channels, 128-byte rows with
-// the 128-byte swizzle; V is read in place as an MN-major operand.
+// are turned into fp16 pairs on the way through registers), warp 12 issues the products, S one tile ahead of P
+// V.  K and V tiles are panels of 64 channels, 128-byte rows with the 128-byte swizzle; V is read in place as an
+// MN-major operand.
 //
 // q enters as fp16 after a scaling by a power of two that brings the row's largest channel to
 // [2^11, 2^12), and P relative to 2^-7 of the running maximum, both as pairs of a high half and what it leaves: 22
 // bits, as the row kernel has, so that the form a call goes through is not seen in its output's low half.
 // (Single halves, 2^-11 of q, move a score by up to 2^-11 sum |q k| / sqrt(D): with loud channels more than
-// the bf16 output rounds off.)  4-bit values round to fp16.  Sums, maxima and O are fp32.
+// the bf16 output rounds off.)  4-bit values are pairs too, to 2^-18 of their group's largest.  Products of two
+// low parts are left out.  Sums, maxima and O are fp32.
 //
-// Bound by, a tile: 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the softmax does around
-// them, next to some 1600 cycles of products at D = 128 (57 an instruction of N = 64 for S, 88 of N = 128 for P V); a
-// launch adds some 7 us before its first products and after its last.  16 heads over 8, D = 128, B200: 8 x 128
-// rows, 4 bits 18.4 us (204 TFLOP/s; single halves: 16.7); 2 x 500 rows under a window of 256, fp16 21.1 us (102
-// TFLOP/s; 19.6).
+// Bound by, a tile of D = 128: fp16 by 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the softmax does
+// around them, next to some 1600 cycles of products (57 an instruction of N = 64 for S, 88 of N = 128 for P V); 4 bits by the
+// products, three for two (2400 cycles; without the third 19.0 us for 20.7), and K and V made fp16 beside
+// them.  A launch adds some 8 us before its first products and after its last.  16 heads over 8, D = 128, B200: 8 x
+// 128 rows after 384, 4 bits 20.7 us (182 TFLOP/s; 16.7 in single halves); 2 x 500 rows under a window of 256,
+// fp16 21.1 us (102 TFLOP/s; 19.6).  4 bits with the scales on P and on S instead, codes alone in the products: 38.8.
 // Every wait is bounded.
 #pragma once
 
@@ -71,10 +73,12 @@ __device__ __forceinline__ bool elect_one() {
 template <int FMT, int D>
 struct ChunkLayout {
     static constexpr int NW = D / 64;
-    static constexpr int ST = FMT == kWinQ4 ? 3 : 4;  // stages of fp16 tiles
-    static constexpr int RAW = FMT == kWinQ4 ? 4 : 0; // tiles of codes on their way (cp.async), before they are turned into fp16
+    static constexpr int NP = FMT == kWinQ4 ? 2 : 1;  // fp16 numbers a value of K or V is held in
+    static constexpr int ST = FMT == kWinQ4 ? 2 : 4;  // stages of fp16 tiles
+    static constexpr int RAW = FMT == kWinQ4 ? 3 : 0; // tiles of codes on their way (cp.async), before they are turned into fp16
     static constexpr int PANEL = 64 * 128;            // 64 keys x 64 channels
-    static constexpr int STAGE = 2 * NW * PANEL;      // K panels, V panels
+    static constexpr int PART_KV = NW * PANEL;        // high or low parts of K or V
+    static constexpr int STAGE = 2 * NP * PART_KV;    // K's parts, V's parts
     static constexpr int QHALF = NW * 128 * 128;      // NW panels of 128 rows
     static constexpr int Q = 0;                       // high halves, low halves
     static constexpr int RING = Q + 2 * QHALF;
@@ -232,8 +236,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         }
         return bad;
     };
-    auto wait_empty = [&](int i) {  // the stage of tile i >= ST has been read
-        ok = mbar_wait(&empty[i % ST], (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
+    // The stage of tile i >= ST has been read.  4 bits: K's, with two stages and two S, once S of tile i - 2 is there; as
+    // softmax may still be at that tile, it waits for nothing of K's loaders (k_full could be two phases on).
+    auto wait_empty = [&](int i) {
+        uint64_t* read = FMT == kWinQ4 && !is_v ? &s_full[i & 1] : &empty[i % ST];
+        ok = mbar_wait(read, (uint32_t)(i / ST - 1) & 1u, DEV_ERR_ATTN_WAIT);
         ok = __all_sync(0xffffffffu, ok);
     };
     // 4 bits: codes through the warp's own ring, RAW - 1 tiles ahead
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     // fp16: 16-byte piece c of this thread's half row of a tile
     auto piece = [&](int st, int c) {
         const int ch = half * (D / 16) + c;  // of D / 8
-        return smem + L::RING + st * L::STAGE + (is_v * NW + (ch >> 3)) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
+        return smem + L::RING + st * L::STAGE + is_v * L::NP * L::PART_KV + (ch >> 3) * L::PANEL + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
     };
     auto fetch = [&](int i) {  // tile i's copies, a group
         const int id = i < nt ? block_id(i) : -1;
@@ -301,7 +308,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                     *reinterpret_cast<uint2*>(smem + L::Q + half * L::QHALF + (c >> 4) * 16384 +
                                               sw128_off(row, (c & 15) * 4)) = x;
                 }
-                if (c == 0) s_sf[row] = __uint_as_float((uint32_t)(ex - 11) << 23) * p.scale_log2;
+                if (c == 0) s_sf[row] = __uint_as_float((uint32_t)(ex - 11) << 23) * (FMT == kWinQ4 ? 2.f * p.scale_log2 : p.scale_log2);
             }
 #pragma unroll
             for (int k = 0; k < 6; ++k) q_now[k] = q_next[k];
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         for (int i = 0; i < nt && ok; ++i) {
             const int st = i % ST, pos = (t0 + i) * 4;
             ok = mbar_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, DEV_ERR_ATTN_WAIT) &&
-                 mbar_wait(&k_full[st], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);  // (for s_here)
+                 mbar_wait(FMT == kWinQ4 ? &v_full[st] : &k_full[st], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT);  // (for s_here)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -405,27 +412,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     } else if (warp < 12) {
         // ------------------------------------------------------------------ K (is_v 0) or V: block `w4` of each tile
         if constexpr (FMT == kWinQ4) {
-            // nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as fp16 pairs, times scale plus zero
-            auto values = [&](uint32_t x, __half2 scale, __half2 zero) {
-                const __half2 k1024 = __floats2half2_rn(1024.f, 1024.f), k16 = __floats2half2_rn(0.0625f, 0.0625f),
-                              k64 = __floats2half2_rn(-64.f, -64.f), k65504 = __floats2half2_rn(65504.f, 65504.f);
-                uint4 u;
-                uint32_t* o = &u.x;
+            // Nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as two fp16 pairs, high + low = half of code * scale + zero (half,
+            // so that values past 65504 fit).  With g = 2^-9 of the power of two below the group's largest value M,
+            // scale and zero are multiples of g (sh, zh) and what those leave (sl, zl): the high part is exact, a
+            // multiple of g / 2 below 2^11 of them, and the low part, below 4 g, rounds: the value is off by at most 2^-18 of
+            // M (2^-23 where M is below 2^-5).
+            auto values = [&](uint32_t x, __half2 sh, __half2 sl, __half2 zh, __half2 zl, uint4& hi, uint4& lo) {
+                uint32_t *oh = &hi.x, *ol = &lo.x;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t y = x >> (8 * h);
-                    const uint32_t a = (y & 0x000f000fu) | 0x64006400u, b = (y & 0x00f000f0u) | 0x64006400u;
-                    const __half2 ca = __hsub2(*reinterpret_cast<const __half2*>(&a), k1024);
-                    const __half2 cb = __hfma2(*reinterpret_cast<const __half2*>(&b), k16, k64);
-                    const __half2 va = __hmin2_nan(__hfma2(ca, scale, zero), k65504),
-                                  vb = __hmin2_nan(__hfma2(cb, scale, zero), k65504);
-                    o[2 * h] = *reinterpret_cast<const uint32_t*>(&va);
-                    o[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&vb);
+                for (int h = 0; h < 4; ++h) {
+                    // 512 + code / 2 is an fp16 number with the nibble in its low bits
+                    const uint32_t a = ((x >> (4 * h)) & 0x000f000fu) | 0x60006000u;
+                    const __half2 c = __hsub2_rn(*reinterpret_cast<const __half2*>(&a), __floats2half2_rn(512.f, 512.f));
+                    const __half2 v = __hfma2(c, sh, zh), l = __hfma2(c, sl, zl);
+                    oh[h] = *reinterpret_cast<const uint32_t*>(&v);
+                    ol[h] = *reinterpret_cast<const uint32_t*>(&l);
                 }
-                return u;
             };
             // a thread's words: i = 4 half + k / NW of group k % NW (k < 4 NW), of a row of D / 8 words
-            uint8_t* to = smem + L::RING + is_v * NW * L::PANEL + key * 128;
+            uint8_t* to = smem + L::RING + is_v * L::NP * L::PART_KV + key * 128;
             const uint32_t from = raw + off * (D / 2) + half * 16 * NW;
             for (int i = 0; i < nt; ++i) {
                 const int st = i % ST;
@@ -434,37 +439,44 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 fetch(i + L::RAW - 1);
                 const bool in = (valid >> (i & 31)) & 1;
                 uint32_t x[NW][4] = {};
-                __half2 scale[NW], zero[NW];
+                const bool check = is_v && hidden(i, in);
+                bool bad = false;
+                __half2 sh[NW], sl[NW], zh[NW], zl[NW];  // scales; zeros' halves
 #pragma unroll
-                for (int c = 0; c < NW; ++c) scale[c] = zero[c] = __floats2half2_rn(0.f, 0.f);
+                for (int c = 0; c < NW; ++c) sh[c] = sl[c] = zh[c] = zl[c] = __floats2half2_rn(0.f, 0.f);
                 if (in) {
                     const uint32_t slot_at = (i % L::RAW) * G::BYTES;
 #pragma unroll
                     for (int c = 0; c < NW; ++c) {
                         lds_words(x[c], from + slot_at + 16 * c);
-                        const float2 prm = lds_half2(raw + slot_at + Q4Layout<D>::PARAMS + c * 64 + off * 4);
-                        scale[c] = __float2half2_rn(prm.x);
-                        zero[c] = __float2half2_rn(prm.y);
+                        float2 prm = lds_half2(raw + slot_at + Q4Layout<D>::PARAMS + c * 64 + off * 4);
+                        // what a key that some row does not see may hold: not what a write leaves
+                        const float top = fmaxf(fabsf(prm.y), fabsf(fmaf(15.f, prm.x, prm.y)));  // M
+                        if (check && !(fabsf(prm.x) <= 8736.f && top < 100000.f)) prm = make_float2(0.f, 0.f), bad = true;
+                        // adding 1.5 * 2^23 g rounds to a multiple of g (2^-23 at least: halves stay fp16 numbers)
+                        const uint32_t e = max((int)(__float_as_uint(top) >> 23), 113);
+                        const float magic = __uint_as_float(((e + 14) << 23) | 0x400000u);
+                        const float s0 = __fsub_rn(__fadd_rn(prm.x, magic), magic), z0 = __fsub_rn(__fadd_rn(prm.y, magic), magic);
+                        sh[c] = __float2half2_rn(s0);
+                        sl[c] = __float2half2_rn(prm.x - s0);
+                        zh[c] = __float2half2_rn(0.5f * z0);
+                        zl[c] = __float2half2_rn(0.5f * (prm.y - z0));
                     }
                 }
                 if (i >= ST) {
                     wait_empty(i);
                     if (!ok) break;
                 }
-                if (!is_v && lane == 0) s_here[st][w4] = in;
-                const bool check = is_v && hidden(i, in);
-                uint4 u[4 * NW];
-#pragma unroll
-                for (int c = 0; c < 4 * NW; ++c) u[c] = values(x[c >> 2][c & 3], scale[c % NW], zero[c % NW]);
-                bool bad = false;
-                if (check) {
-#pragma unroll
-                    for (int c = 0; c < 4 * NW; ++c) bad |= clean(u[c]);
-                }
+                if (is_v && lane == 0) s_here[st][w4] = in;
 #pragma unroll
                 for (int c = 0; c < 4 * NW; ++c) {  // channels 64 w + 8 ii .. + 7, w = c % NW
                     const int ii = 4 * half + c / NW;
-                    *reinterpret_cast<uint4*>(to + st * L::STAGE + (c % NW) * L::PANEL + ((ii ^ (key & 7)) << 4)) = u[c];
+                    uint4 u[2];
+                    values(x[c >> 2][c & 3], sh[c % NW], sl[c % NW], zh[c % NW], zl[c % NW], u[0], u[1]);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+                        *reinterpret_cast<uint4*>(to + st * L::STAGE + part * L::PART_KV + (c % NW) * L::PANEL +
+                                                  ((ii ^ (key & 7)) << 4)) = u[part];
                 }
                 if (is_v) {
                     s_bad[st][pt] = bad;
@@ -509,24 +521,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
         const uint32_t idesc_s = make_idesc_f16(128, 64), idesc_o = make_idesc_f16(128, D) | (1u << 16);  // V is MN-major
         // descriptors of the buffers' starts; a step's is an addition to the address field (16-byte units)
         const uint64_t q_desc = make_sw128_desc(smem_u32(smem + L::Q)), k_desc = make_sw128_desc(smem_u32(smem + L::RING)),
-                       v_desc = make_sw128_mn_desc(smem_u32(smem + L::RING + NW * L::PANEL), L::PANEL);
+                       v_desc = make_sw128_mn_desc(smem_u32(smem + L::RING + L::NP * L::PART_KV), L::PANEL);
         auto issue_s = [&](int i) {
-            if (!mbar_wait(&k_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT)) return false;
+            // (every lane has waited before one issues: K's next tile may follow the products at once)
+            if (!__all_sync(0xffffffffu, mbar_wait(&k_full[i % ST], (uint32_t)(i / ST) & 1u, DEV_ERR_ATTN_WAIT))) return false;
             tc_fence_after();
             const uint64_t kd = k_desc + (uint32_t)((i % ST) * (L::STAGE >> 4));
             const uint32_t d = tmem + L::TS + (i & 1) * 64;
             if (lead) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int t = 0; t < 1 + L::NP; ++t)  // both halves of q times K, the high one times K's low parts
 #pragma unroll
                     for (int kk = 0; kk < 4 * NW; ++kk)
-                        umma_bf16(d, q_desc + (half * (L::QHALF >> 4) + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3)),
-                                  kd + ((kk >> 2) * (L::PANEL >> 4) + 2 * (kk & 3)), idesc_s, (half | kk) ? 1u : 0u);
+                        umma_bf16(d, q_desc + ((t & 1) * (L::QHALF >> 4) + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3)),
+                                  kd + ((t >> 1) * (L::PART_KV >> 4) + (kk >> 2) * (L::PANEL >> 4) + 2 * (kk & 3)), idesc_s,
+                                  (t | kk) ? 1u : 0u);
                 umma_commit(&s_full[i & 1]);
             }
             return true;
         };
-        if (nt > 0) ok = mbar_wait(&q_full, 0, DEV_ERR_ATTN_WAIT) && issue_s(0);
+        if (nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0, DEV_ERR_ATTN_WAIT)) && issue_s(0);
         for (int i = 0; i < nt && ok; ++i) {
             if (i + 1 < nt) ok = issue_s(i + 1);
             ok = ok && mbar_wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u, DEV_ERR_ATTN_WAIT);
@@ -538,11 +552,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
             const uint32_t pt0 = tmem + L::TP + (i & 1) * 64;
             if (lead) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int t = 0; t < 1 + L::NP; ++t)  // both halves of P times V, the high one times V's low parts
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma_ts_f16(tmem + L::TO, pt0 + half * 32 + kk * 8, vd + kk * (2048 >> 4), idesc_o,
-                                    (i > 0 || half > 0 || kk > 0) ? 1u : 0u);
+                        umma_ts_f16(tmem + L::TO, pt0 + (t & 1) * 32 + kk * 8,
+                                    vd + (t >> 1) * (L::PART_KV >> 4) + kk * (2048 >> 4), idesc_o,
+                                    (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(&empty[i % ST]);
                 umma_commit(&pv_done[i & 1]);
             }
@@ -567,7 +582,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     if (warp < 4) {
         const uint32_t lanes = tmem + ((uint32_t)warp << 21) + L::TO;
         const bool sum = ok && nt > 0 && l != 0.f;  // else zeros (NaN counts as a sum)
-        const float inv = splits == 1 ? 1.f / l : 1.f;
+        const float inv = (FMT == kWinQ4 ? 2.f : 1.f) * (splits == 1 ? 1.f / l : 1.f);  // (4 bits: V is halved)
         uint8_t* staged = smem + L::RING;  // [row][ROWB] bf16, then the low halves
         s_part[r][0] = m;
         s_part[r][1] = ok ? l : 0.f;

@@ -109,7 +109,7 @@ def _chunk(fmt, S, past, Hq, H, D, qscale, seed=0):
     return got[list(rows)], want, np.sqrt((kv[1] ** 2).mean())
 
 
-@pytest.mark.parametrize("fmt", ["fp16"])
+@pytest.mark.parametrize("fmt", ["q4", "fp16"] if FORCED == "1" else ["fp16"])
 @pytest.mark.parametrize("Hq,H,D", [(4, 2, 128), (8, 2, 64)])
 @pytest.mark.parametrize("S,past,qscale", [(150, 3, 1.0), (150, 100, 4.0), (70, 900, 2.0)])
 def test_chunks_keep_sixteen_bits(fmt, Hq, H, D, S, past, qscale):
