@@ -18,10 +18,10 @@
 // runs at once, a block to a lane; for P V each block takes its own group's columns of P, the opposite
 // group's hold the low parts, the rest zero.  The column groups of O add up at the end.
 //
-// 4-bit pool, K: the nibbles of a word are two words of bytes, (x << 4) & 0xf0f0f0f0 and x &
-// 0xf0f0f0f0, both 16 code: unsigned operands of an integer product (m16n8k32).  q is a 16-bit
-// fixed-point number in two signed digits, its unit 2^-16 of the slot's largest channel (far below the
-// error of a 4-bit key); the sum is exact.  A key's scale multiplies the sum, its zero sum(q).
+// 4-bit pool, K: the nibbles of a word are two words of bytes, x & 0x0f0f0f0f and (x >> 4) & 0x0f0f0f0f: unsigned
+// operands of an integer product (m16n8k32).  q is a 22-bit fixed-point number in three signed digits, its unit
+// 2^-21 of the slot's largest channel (two digits, 2^-16, moved scores by up to 1e-4 where q has loud channels);
+// 64 codes of 15 times it stay below 2^31, so that the sum is exact.  A key's scale multiplies the sum, its zero sum(q).
 // V: a nibble masked out of a code word IS a small bf16 number (a subnormal: nibble << 0 = code *
 // 2^-133, nibble << 4 = 16 times that), so that no conversion is needed; the powers of two move
 // into p and the output, a token's scale into its probability, and its zero is added on the fp32 side.
@@ -187,9 +187,9 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_ml[W][SL][2];
     __shared__ float s_part[SL][2];  // the CTA's (max, sum) per slot
-    // Q^T operand words of (slot, t): high parts, then low parts; accumulator -> log2 units; sums of q
-    constexpr int NQ = FMT == kWinQ4 ? 2 * NW : MT;
-    __shared__ __align__(16) uint32_t s_q[SL][4][4 * NQ];
+    // Q^T operand words of (slot, t): high parts to low parts; accumulator -> log2 units; sums of q
+    constexpr int NQ = FMT == kWinQ4 ? 2 * NW : MT, QP = FMT == kWinQ4 ? 3 : 2;
+    __shared__ __align__(16) uint32_t s_q[SL][4][QP * 2 * NQ];
     __shared__ float s_qf[SL], s_qsum[SL][NW];
     static_assert(SL * D * 4 <= RING, "a warp's partial output replaces its ring");
 
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
     // Q^T operand, made once per CTA.
     //   fp16: q scaled by a power of two that brings the slot's largest channel to [2^11, 2^12), so
     //   that two fp16 halves hold it whatever its size.
-    //   4 bits: q / (largest channel) * 32639 rounded to an integer = 256 high + low, digits in [-128, 127].
+    //   4 bits: q / (largest channel) * 2^21 rounded to an integer, digits of 65536, 256 and 1, the lower two in [-128, 127].
 #pragma unroll
     for (int k = 0; k < QS; ++k) {
         const int s = warp + k * W;
@@ -322,24 +322,26 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
         if constexpr (FMT == kWinQ4) {
             // a q that is zero everywhere (or below what a reciprocal holds) scores zero; one that is
             // not finite makes its scores NaN through f
-            const float up = amax >= 1e-30f ? 32639.f / amax : 0.f;
-            f = amax * (1.f / (32639.f * 16.f)) * p.scale_log2;
+            const float up = amax >= 1e-30f ? 2097152.f / amax : 0.f;
+            f = amax * (1.f / 2097152.f) * p.scale_log2;
             if (!(amax < INFINITY)) f = __int_as_float(0x7fffffff);
             float sum = (qv[k][0] + qv[k][1]) + (qv[k][2] + qv[k][3]);
 #pragma unroll
             for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            uint32_t hi = 0, lo = 0;
+            uint32_t hi = 0, mid = 0, lo = 0;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int x = __float2int_rn(qv[k][c] * up), h = (x + 128) >> 8;
+                const int x = __float2int_rn(qv[k][c] * up), y = (x + 128) >> 8, h = (y + 128) >> 8;
                 hi |= (uint32_t)(h & 255) << (8 * c);
-                lo |= (uint32_t)((x - 256 * h) & 255) << (8 * c);
+                mid |= (uint32_t)((y - 256 * h) & 255) << (8 * c);
+                lo |= (uint32_t)((x - 256 * y) & 255) << (8 * c);
             }
             const int w = lane >> 4;
             if (w < NW) {
                 uint32_t* dst = &s_q[s][(lane >> 2) & 3][2 * (2 * w + (lane & 1)) + ((lane >> 1) & 1)];
                 dst[0] = hi;
-                dst[2 * NQ] = lo;
+                dst[2 * NQ] = mid;
+                dst[4 * NQ] = lo;
                 if ((lane & 15) == 0) s_qsum[s][w] = sum * p.scale_log2;
             }
         } else {
@@ -358,14 +360,15 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
         if (lane == 0) s_qf[s] = f;
     }
     __syncthreads();
-    uint32_t qh[NQ][2], ql[NQ][2];     // of column g: slot g % SL
+    uint32_t qh[NQ][2], qm[FMT == kWinQ4 ? NQ : 1][2], ql[NQ][2];  // of column g: slot g % SL
     float sf[2], qsum[NW][2];          // of this lane's score columns
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             qh[i][h] = s_q[g % SL][t][2 * i + h];
-            ql[i][h] = s_q[g % SL][t][2 * NQ + 2 * i + h];
+            if constexpr (FMT == kWinQ4) qm[i][h] = s_q[g % SL][t][2 * NQ + 2 * i + h];
+            ql[i][h] = s_q[g % SL][t][2 * NQ * (QP - 1) + 2 * i + h];
         }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
                     lds_words(kw[k][1], buf + (k0 + k) * G::BYTES + sw + 8 * (D / 2));
                 }
                 int d[KI][NW][4];
-                uint32_t a[2][KI][NW][4];  // even and odd nibbles, times 16
+                uint32_t a[2][KI][NW][4];  // even and odd nibbles
 #pragma unroll
                 for (int k = 0; k < KI; ++k)
 #pragma unroll
@@ -430,20 +433,20 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_window_kernel(const W
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint32_t x = kw[k][i & 1][(i >> 1) * NW + w];
-                            a[0][k][w][i] = (x << 4) & 0xf0f0f0f0u;
-                            a[1][k][w][i] = x & 0xf0f0f0f0u;
+                            a[0][k][w][i] = x & 0x0f0f0f0fu;
+                            a[1][k][w][i] = (x >> 4) & 0x0f0f0f0fu;
                         }
 #pragma unroll
-                for (int step = 0; step < 4; ++step)  // high digits of both nibbles, then low ones
+                for (int step = 0; step < 6; ++step)  // high digits of both nibbles, then lower ones
 #pragma unroll
                     for (int k = 0; k < KI; ++k)
 #pragma unroll
                         for (int w = 0; w < NW; ++w) {
-                            if (step == 2)
+                            if (step == 2 || step == 4)
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) d[k][w][i] *= 256;
                             if (step == 0) mma_u8s8_first(d[k][w], a[0][k][w], qh[2 * w]);
-                            else mma_u8s8(d[k][w], a[step & 1][k][w], step < 2 ? qh[2 * w + 1] : ql[2 * w + (step & 1)]);
+                            else mma_u8s8(d[k][w], a[step & 1][k][w], (step < 2 ? qh : step < 4 ? qm : ql)[2 * w + (step & 1)]);
                         }
 #pragma unroll
                 for (int k = 0; k < KI; ++k)

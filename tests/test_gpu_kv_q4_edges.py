@@ -109,7 +109,7 @@ def _chunk(fmt, S, past, Hq, H, D, qscale, seed=0):
     return got[list(rows)], want, np.sqrt((kv[1] ** 2).mean())
 
 
-@pytest.mark.parametrize("fmt", ["q4", "fp16"] if FORCED == "1" else ["fp16"])
+@pytest.mark.parametrize("fmt", ["q4", "fp16"])
 @pytest.mark.parametrize("Hq,H,D", [(4, 2, 128), (8, 2, 64)])
 @pytest.mark.parametrize("S,past,qscale", [(150, 3, 1.0), (150, 100, 4.0), (70, 900, 2.0)])
 def test_chunks_keep_sixteen_bits(fmt, Hq, H, D, S, past, qscale):
@@ -121,6 +121,31 @@ def test_chunks_keep_sixteen_bits(fmt, Hq, H, D, S, past, qscale):
     got, want, rms_v = _chunk(fmt, S, past, Hq, H, D, qscale)
     err = np.sqrt(((got - want) ** 2).mean(-1))
     assert err.max() <= 2.0 ** -16 * (1 + qscale) * rms_v, err.max() / rms_v
+
+
+@pytest.mark.parametrize("Hq,H,D", [(16, 8, 128), (16, 4, 128), (16, 2, 128), (6, 2, 64), (4, 1, 64)])
+@pytest.mark.parametrize("ctx,qscale", [(9, 1.0), (300, 4.0), (2000, 2.0)])
+def test_decode_rows_keep_sixteen_bits_over_4_bits(Hq, H, D, ctx, qscale):
+    """Decode rows whose q has a channel 30 times as loud as the rest, against the bound of the test above: the loud
+    channel is 30 qscale, so that q is off by 2^-22 * 30 qscale a channel, 2^-17 qscale |k| / sqrt(D) of a score at the very
+    most.  Its scores alone are large, so its K channel is 1/16 of the others'."""
+    rows, nb = 5, -(-ctx // 16)
+    x = torch.randn(nb, 1, 2, H, 16, D, generator=_gen(21))
+    x[:, :, 0, :, :, 5] /= 16
+    raw = O.pack(*O.quantise(x.half().float().numpy()))
+    kv = O.unpack(raw)[:, 0].transpose(1, 2, 0, 3, 4).reshape(2, H, -1, D)
+    q = torch.randn(rows, Hq, D, generator=_gen(22)) * qscale
+    q[:, :, 5] = 30 * qscale
+    zero = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    lo = torch.empty(rows, Hq * D, device=DEV, dtype=torch.bfloat16)
+    out = ops.paged_attention_q4(q.to(DEV), torch.from_numpy(raw).to(DEV), 0,
+                                 torch.arange(nb, dtype=torch.int32, device=DEV).view(1, nb), zero, zero + ctx, ctx,
+                                 out_lo=lo)
+    got = (out.double() + lo.double()).cpu().numpy()
+    rms_v = np.sqrt((kv[1] ** 2).mean())
+    for r in range(rows):
+        want = O.attention(q[r].numpy(), kv[0], kv[1], ctx)
+        assert np.sqrt(((got[r] - want) ** 2).mean()) <= 2.0 ** -16 * (1 + qscale) * rms_v, r
 
 
 # ------------------------------------------------------------------------------ the cache
