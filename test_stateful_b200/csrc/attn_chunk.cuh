@@ -681,56 +681,118 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// Whether rows go through 128-row tiles (QTTS_WINDOW_TILES=0 / 1 forces it where either form can run).
-// A tile CTA costs some 7 us before its first products and after its last, the row kernel 8 rows' reading
-// of every block; tiles win once they are at least half full and the row kernel has more than a few
-// thousand (8-row tile, block) pairs or more than a wave of tiles.  Measured (us, 16 heads over 8,
-// streams x rows + past, tiles / rows, B200):
-//   4 bits  1 x 64 + 500   13.3 / 8.9     1 x 128 + 500  13.5 / 12.7   1 x 256 + 500  15.0 / 22.2
-//           8 x 16 + 500   14.1 / 12.3    8 x 32 + 500   14.9 / 18.9   8 x 64 + 500   16.8 / 33.5
-//           2 x 64          9.0 / 7.1     8 x 64          9.2 / 12.7   1 x 1000 + 4000  92 / 343
-//           1 x 16 + 8000  26.1 / 18.2    1 x 32 + 8000  26.8 / 28.0   1 x 64 + 8000  29.0 / 48.9
-//   fp16    1 x 64 + 500   14.9 / 13.1    1 x 128 + 500  15.1 / 14.1   1 x 256 + 500  16.6 / 24.1
-//           8 x 16 + 500   16.6 / 13.3    8 x 32 + 500   17.5 / 20.5   8 x 64 + 500   19.4 / 39.7
-//           1 x 32 + 8000  39.5 / 29.3    1 x 64 + 8000  41.5 / 49.2   1 x 1000 + 4000 160 / 351
-inline bool use_chunk_kernel(const WinParams& p) {
+// CTAs of clusters of `splits` that are on the card at once (the clusters of eight are fewer than its SMs hold CTAs,
+// as a cluster stays within a GPC: 16 of them ran as two waves).  Asked once per kernel, device and size.
+template <int FMT, int D>
+inline int chunk_clusters(int splits) {
+    constexpr auto kernel = paged_attn_chunk_kernel<FMT, D>;
+    static std::atomic<int> known[64][4];
+    int dev = 0, n = 0, at = 0;
+    while ((1 << at) < splits) ++at;  // 1, 2, 4, 8
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64 && (n = known[dev][at].load(std::memory_order_relaxed)) > 0) return n;
+    if (func_attr_once<kernel>(ChunkLayout<FMT, D>::SMEM) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits);
+    cfg.blockDim = dim3(kChunkThreads);
+    cfg.dynamicSmemBytes = ChunkLayout<FMT, D>::SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (dev < 64) known[dev][at].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+// How a call would go through 128-row tiles: queries a tile, tiles of a stream and of all, the CTAs that share a
+// tile's keys (while all clusters are on the card at once and a CTA keeps two tiles), 64-key tiles a CTA walks.
+struct ChunkPlan {
+    int qt, stream_tiles, splits, walk;
+    long long tiles;
+};
+// keys that a tile of `q` queries reads, at most
+inline long long window_keys(const WinParams& p, int q) {
+    const long long limit = p.max_ctx < p.mbps * 16 ? p.max_ctx : p.mbps * 16, seen = (long long)p.window + p.sinks + q + 32;
+    return p.window > 0 && seen < limit ? seen : limit;
+}
+template <int FMT, int D>
+inline ChunkPlan plan_chunk(const WinParams& p) {
+    ChunkPlan c;
+    c.qt = 128 / p.group < p.S ? 128 / p.group : p.S;
+    c.stream_tiles = ceil_div(p.S, c.qt);
+    c.tiles = (long long)(p.R / p.S) * c.stream_tiles * p.kv_heads;
+    const long long keys = window_keys(p, c.qt);
+    c.splits = 1;
+    while (c.splits < 8 && keys >= 2ll * c.splits * 2 * 64 && c.tiles <= chunk_clusters<FMT, D>(c.splits * 2)) c.splits *= 2;
+    c.walk = (int)((keys + 64 * c.splits - 1) / (64 * c.splits));
+    return c;
+}
+
+// Whether rows go through 128-row tiles (QTTS_WINDOW_TILES=0 / 1 forces it where either form can run): the shorter of
+// two estimates in us, fitted to 192 measured pairs (four head layouts, both pools, 1 to 16 streams of 16 to 1000 rows, 0
+// to 8000 keys before them; the pick is within 11% of the better form, once 19%).
+//   tiles:      waves (8 + c a 64-key tile of a CTA), 3 more for a cluster; c = 1.4 (4 bits), 2.3 (fp16), D = 64: 1.0, 1.2
+//   8-row tiles: 5 + 6.6e-6 D a (tile, 16-key block) pair + 3e-3 (4 bits) or 8e-3 (fp16) a tile
+// Measured (us, 16 heads over 8, D = 128, streams x rows + past, tiles / 8-row tiles, B200, K and V from HBM):
+//   4 bits  1 x 64 + 500   14.8 / 9.2     1 x 128 + 500  15.1 / 13.3   1 x 256 + 500  16.3 / 23.4
+//           8 x 16 + 500   16.5 / 12.8    8 x 32 + 500   17.5 / 19.8   8 x 64 + 500   19.4 / 35.5
+//           2 x 64         10.2 / 7.1     8 x 64         10.3 / 12.9   1 x 1000 + 4000 119 / 370
+//           1 x 16 + 8000  33.3 / 19.5    1 x 32 + 8000  34.0 / 30.4   1 x 64 + 8000  36.2 / 52.8
+//   fp16    1 x 64 + 500   15.8 / 13.9    1 x 128 + 500  16.1 / 15.0   1 x 256 + 500  17.6 / 25.1
+//           8 x 16 + 500   18.9 / 14.6    8 x 32 + 500   19.8 / 21.9   8 x 64 + 500   21.6 / 41.9
+//           2 x 64         10.3 / 8.6     8 x 64         10.5 / 20.2   1 x 1000 + 4000 191 / 374
+//           1 x 16 + 8000  45.2 / 21.2    1 x 32 + 8000  45.7 / 31.1   1 x 64 + 8000  47.9 / 52.1
+// The keys are max_ctx's (contexts are on the device): a bound far above them picks the wrong form at times.
+template <int FMT, int D>
+inline bool use_chunk_kernel(const WinParams& p, const ChunkPlan& c) {
     static const int forced = [] {
         const char* v = getenv("QTTS_WINDOW_TILES");
         return v && (v[0] == '0' || v[0] == '1') ? v[0] - '0' : -1;
     }();
-    if (p.S < 2 || p.group > 128) return false;
-    if (((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_lo)) & 15) != 0) return false;
     if (forced >= 0) return forced == 1;
-    const long long heads = (long long)(p.R / p.S) * p.kv_heads, rows = (long long)p.S * p.group;
-    if (rows < 64 || (rows < 128 && heads < 16)) return false;
+    const long long heads = (long long)(p.R / p.S) * p.kv_heads;
     const long long row_tiles = heads * (p.group >= 8 ? (long long)p.S * ceil_div(p.group, 8) : ceil_div(p.S, 8 / p.group));
-    long long keys = p.max_ctx;
-    if (p.window > 0 && (long long)p.window + p.sinks + 32 < keys) keys = (long long)p.window + p.sinks + 32;
-    return row_tiles > 4 * num_sms() || row_tiles * (keys / 16) >= 8192;
+    const double waves = c.splits > 1 ? 1. : (double)((c.tiles + num_sms() - 1) / num_sms());
+    const double a_tile = FMT == kWinQ4 ? (D == 128 ? 1.4 : 1.0) : (D == 128 ? 2.3 : 1.2);
+    const double tiles_us = waves * (8. + a_tile * c.walk) + (c.splits > 1 ? 3. : 0.);
+    const double rows_us = 5. + 6.6e-6 * D * ((double)row_tiles * (double)(window_keys(p, 8) / 16.)) +
+                           (FMT == kWinQ4 ? 3e-3 : 8e-3) * (double)row_tiles;
+    return tiles_us < rows_us;
 }
 
 template <int FMT, int D>
-inline int launch_chunk_attention(WinParams p, cudaStream_t st) {
+inline int launch_chunk_attention(WinParams p, const ChunkPlan& c, cudaStream_t st) {
     using L = ChunkLayout<FMT, D>;
     using G = WinChunk<FMT, D>;
-    p.qt = 128 / p.group < p.S ? 128 / p.group : p.S;
-    p.tiles = ceil_div(p.S, p.qt);
+    p.qt = c.qt;
+    p.tiles = c.stream_tiles;
     const long long block_bytes = (long long)p.num_layers * 2 * p.kv_heads * G::BYTES;
     QTTS_REQUIRE(block_bytes < (1ll << 31), "paged attention: %lld bytes per block", block_bytes);
     p.block_bytes = (uint32_t)block_bytes;
     p.v_offset = (uint32_t)(p.kv_heads * G::BYTES);
-    const long long tiles = (long long)(p.R / p.S) * p.tiles * p.kv_heads;
-    QTTS_REQUIRE(tiles * 8 < (1ll << 31), "paged attention: %lld tiles", tiles);
-    const int limit = p.max_ctx < p.mbps * 16 ? p.max_ctx : p.mbps * 16;
-    long long keys = limit;
-    if (p.window > 0 && (long long)p.window + p.sinks + p.qt + 32 < keys) keys = (long long)p.window + p.sinks + p.qt + 32;
-    // a cluster shares the keys of a tile while all CTAs have an SM of their own and two tiles each
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= num_sms() && keys >= 2ll * splits * 2 * 64) splits *= 2;
+    QTTS_REQUIRE(c.tiles * 8 < (1ll << 31), "paged attention: %lld tiles", c.tiles);
     constexpr auto kernel = paged_attn_chunk_kernel<FMT, D>;
     QTTS_CHECK_CUDA((func_attr_once<kernel>(L::SMEM)));
-    QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(tiles * splits)), dim3(kChunkThreads), L::SMEM, st, dim3(splits, 1, 1), p));
+    QTTS_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(c.tiles * c.splits)), dim3(kChunkThreads), L::SMEM, st,
+                               dim3(c.splits, 1, 1), p));
     return QTTS_OK;
+}
+
+// Decode rows, and chunks in the form that suits them.
+template <int FMT, int D>
+inline int launch_attention(const WinParams& p, cudaStream_t st) {
+    const bool either = p.S > 1 && p.group <= 128 &&
+                        ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_lo)) & 15) == 0;
+    if (either) {
+        const ChunkPlan c = plan_chunk<FMT, D>(p);
+        if (use_chunk_kernel<FMT, D>(p, c)) return launch_chunk_attention<FMT, D>(p, c, st);
+    }
+    return launch_window_attention<FMT, D>(p, st);
 }
 
 }  // namespace qtts

@@ -107,14 +107,8 @@ static int window_attention(const char* what, int fmt, const void* q, int R, int
     p.window = window;
     p.sinks = sinks;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
-    if (use_chunk_kernel(p)) {
-        if (fmt == kWinQ4)
-            return head_dim == 128 ? launch_chunk_attention<kWinQ4, 128>(p, st) : launch_chunk_attention<kWinQ4, 64>(p, st);
-        return head_dim == 128 ? launch_chunk_attention<kWinF16, 128>(p, st) : launch_chunk_attention<kWinF16, 64>(p, st);
-    }
-    if (fmt == kWinQ4)
-        return head_dim == 128 ? launch_window_attention<kWinQ4, 128>(p, st) : launch_window_attention<kWinQ4, 64>(p, st);
-    return head_dim == 128 ? launch_window_attention<kWinF16, 128>(p, st) : launch_window_attention<kWinF16, 64>(p, st);
+    if (fmt == kWinQ4) return head_dim == 128 ? launch_attention<kWinQ4, 128>(p, st) : launch_attention<kWinQ4, 64>(p, st);
+    return head_dim == 128 ? launch_attention<kWinF16, 128>(p, st) : launch_attention<kWinF16, 64>(p, st);
 }
 
 }  // namespace qtts
