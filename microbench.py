@@ -13,8 +13,10 @@ achieved bandwidth over the kernel's algorithmic bytes:
 * attention: K+V bytes of every visible key of one layer (fp16) + q/out;
 * gemm: the weight bytes (bf16) + activation hi/lo operands + fp32 output;
 * window-attention: K+V bytes of every key some row of a stream sees (fp16 or 4.5 bits) + q/out;
-* kv-q4: 28 layers of a prompt's K/V quantised into a 4-bit pool, then read back (fp16 rows + pool bytes, each way).
-Inputs cycle through enough copies that every launch reads from HBM.  The
+* kv-q4: 28 layers of a prompt's K/V quantised into a 4-bit pool, then read back (fp16 rows + pool bytes, each way);
+  ``--scattered``: one layer of a decode step's rows, a token in each of so many blocks.
+Inputs (rows, pools, layers of a pool) cycle through enough copies, more than twice L2 together, that every launch
+reads from HBM.  The
 same command is the small case for an ``ncu --set full`` capture.
 """
 
@@ -165,9 +167,11 @@ def _graph_time(launch, launches: int) -> float:
 
 
 def bench_window_attention(fmt: str, rows: int, rows_per_stream: int, ctx_mean: int, spread: float, window: int,
-                           sinks: int, launches: int, layers: int = 4, seed: int = 0):
+                           sinks: int, launches: int, max_ctx: int = 0, heads: int = 16, kv_heads: int = 8, D: int = 128,
+                           seed: int = 0):
     """Windowed attention over the fp16 pool or the 4-bit one: ``rows`` streams of ``rows_per_stream``
-    consecutive rows, contexts U[mean (1 - spread), mean (1 + spread)]."""
+    consecutive rows, contexts U[mean (1 - spread), mean (1 + spread)]; ``max_ctx``: the bound that the call is given
+    (0: the longest context's), as a host that captures a graph gives its pool's."""
     dev = "cuda"
     g = torch.Generator().manual_seed(seed)
     S = rows_per_stream
@@ -175,45 +179,59 @@ def bench_window_attention(fmt: str, rows: int, rows_per_stream: int, ctx_mean: 
     ctx = torch.randint(lo, hi + 1, (rows,), generator=g)
     mbps = -(-hi // 16)
     total = rows * mbps
-    if fmt == "q4":
-        pool = torch.zeros(total, layers, 2, 8, 9 * 128, dtype=torch.uint8, device=dev)
-        m = torch.arange(total * 16, dtype=torch.int32, device=dev)
-        for l in range(layers):
-            kv = torch.randn(2, total * 16, 8, 128, device=dev, dtype=torch.float16)
-            ops.kv_write_q4(pool, kv[0], kv[1], m, layer=l)
-    else:
-        pool = torch.randn(total, layers, 2, 8, 16, 128, device=dev, dtype=torch.float16)
-    table = torch.randperm(total, generator=g).to(torch.int32).view(rows, mbps).to(dev)
-    q = torch.randn(rows * S, 16, 128, generator=g).to(dev)
-    row_slot = torch.arange(rows, dtype=torch.int32).repeat_interleave(S).to(dev)
-    row_ctx = (ctx[:, None] - S + 1 + torch.arange(S)[None, :]).flatten().to(torch.int32).to(dev)
-    out = torch.empty(rows * S, 16 * 128, device=dev, dtype=torch.bfloat16)
-    attend = ops.paged_attention_q4 if fmt == "q4" else ops.paged_attention_window
-    sec = _graph_time(lambda i: attend(q, pool, i % layers, table, row_slot, row_ctx, mbps * 16, window=window,
-                                       sinks=sinks, rows_per_stream=S, out=out), launches)
     w = window or 1 << 30
     keys = sum(min(c, min(c, w + S - 1) + min(sinks, max(0, c - w - S + 1))) for c in ctx.tolist())
-    algo = keys * 2 * 8 * (72 if fmt == "q4" else 256) + rows * S * 16 * 128 * (4 + 2)
+    per_layer = keys * 2 * kv_heads * D * (9 if fmt == "q4" else 32) // 16
+    layers = min(max(4, -(-300_000_000 // per_layer)), max(4, 40_000_000_000 // (total * 2 * kv_heads * D * 32)))
+    launches = max(launches, layers)
+    if fmt == "q4":
+        pool = torch.zeros(total, layers, 2, kv_heads, 9 * D, dtype=torch.uint8, device=dev)
+        m = torch.arange(total * 16, dtype=torch.int32, device=dev)
+        kv = torch.randn(2, total * 16, kv_heads, D, device=dev, dtype=torch.float16)
+        for l in range(layers):
+            ops.kv_write_q4(pool, kv[0], kv[1], m, layer=l)
+    else:
+        pool = torch.randn(total, layers, 2, kv_heads, 16, D, device=dev, dtype=torch.float16)
+    table = torch.randperm(total, generator=g).to(torch.int32).view(rows, mbps)
+    bound = max(max_ctx, mbps * 16)
+    table = torch.nn.functional.pad(table, (0, -(-bound // 16) - mbps), value=-1).contiguous().to(dev)
+    q = torch.randn(rows * S, heads, D, generator=g).to(dev)
+    row_slot = torch.arange(rows, dtype=torch.int32).repeat_interleave(S).to(dev)
+    row_ctx = (ctx[:, None] - S + 1 + torch.arange(S)[None, :]).flatten().to(torch.int32).to(dev)
+    out = torch.empty(rows * S, heads * D, device=dev, dtype=torch.bfloat16)
+    attend = ops.paged_attention_q4 if fmt == "q4" else ops.paged_attention_window
+    sec = _graph_time(lambda i: attend(q, pool, i % layers, table, row_slot, row_ctx, bound, window=window,
+                                       sinks=sinks, rows_per_stream=S, out=out), launches)
+    algo = per_layer + rows * S * heads * D * (4 + 2)
     return {"kernel": "paged attention, window + sinks", "kv": fmt, "streams": rows, "rows_per_stream": S,
-            "window": window, "sinks": sinks, "keys": keys, "launch_us": sec * 1e6, "algorithmic_bytes": algo,
+            "window": window, "sinks": sinks, "keys": keys, "heads": [heads, kv_heads, D], "max_ctx": bound, "layers": layers, "launch_us": sec * 1e6, "algorithmic_bytes": algo,
             "achieved_gbs": algo / sec / 1e9}
 
 
-def bench_kv_q4(tokens: int, launches: int, layers: int = 28):
+def bench_kv_q4(tokens: int, launches: int, dtype: str = "float16", scattered: bool = False):
     dev = "cuda"
-    sets = max(2, -(-300_000_000 // (tokens * layers * 2 * 8 * 128 * 2)))  # > 2x L2 of distinct rows
-    nb = -(-tokens // 16)
-    kv = [torch.randn(tokens, layers, 2, 8, 128, device=dev, dtype=torch.float16) for _ in range(sets)]
-    pool = torch.zeros(nb, layers, 2, 8, 9 * 128, dtype=torch.uint8, device=dev)
-    m = torch.randperm(nb * 16)[:tokens].sort().values.to(torch.int32).to(dev)
-    outs = [torch.empty(2, tokens, layers, 8, 128, device=dev, dtype=torch.float16) for _ in range(sets)]
-    t_w = _graph_time(lambda i: ops.kv_write_q4(pool, kv[i % sets][:, :, 0], kv[i % sets][:, :, 1], m), launches)
-    t_r = _graph_time(lambda i: ops.kv_read_q4(pool, m, n_layers=layers, k=outs[i % sets][0], v=outs[i % sets][1]),
-                      launches)
+    dt = getattr(torch, dtype)
+    layers, nb = (1, tokens) if scattered else (28, -(-tokens // 16))
     values = tokens * layers * 2 * 8 * 128
-    algo = values * 2 + values // 2 + values // 16
-    return {"kernel": "kv_write_q4_kernel / kv_read_q4_kernel", "tokens": tokens, "layers": layers,
-            "write_us": t_w * 1e6, "read_us": t_r * 1e6, "algorithmic_bytes_each": algo,
+    # distinct rows and pools of more than twice L2 each
+    sets = max(2, -(-300_000_000 // (values * dt.itemsize)))
+    pools = min(max(2, -(-300_000_000 // (values * 9 // 16))), 2048)
+    launches = max(launches, sets, pools)
+    kv = torch.randn(sets, tokens, layers, 2, 8, 128, device=dev, dtype=dt)
+    pool = torch.zeros(pools, nb, layers, 2, 8, 9 * 128, dtype=torch.uint8, device=dev)
+    if scattered:  # a token in each block, at uneven offsets
+        m = (torch.randperm(nb) * 16 + torch.randint(0, 16, (nb,))).to(torch.int32).to(dev)
+    else:
+        m = torch.randperm(nb * 16)[:tokens].sort().values.to(torch.int32).to(dev)
+    outs = torch.empty(sets, 2, tokens, layers, 8, 128, device=dev, dtype=dt)
+    t_w = _graph_time(lambda i: ops.kv_write_q4(pool[i % pools], kv[i % sets][:, :, 0], kv[i % sets][:, :, 1], m), launches)
+    for i in range(pools):
+        ops.kv_write_q4(pool[i], kv[0][:, :, 0], kv[0][:, :, 1], m)
+    t_r = _graph_time(lambda i: ops.kv_read_q4(pool[i % pools], m, n_layers=layers, k=outs[i % sets][0],
+                                               v=outs[i % sets][1]), launches)
+    algo = values * dt.itemsize + values // 2 + values // 16
+    return {"kernel": "kv_write_q4_kernel / kv_read_q4_kernel", "tokens": tokens, "layers": layers, "dtype": dtype,
+            "scattered": scattered, "write_us": t_w * 1e6, "read_us": t_r * 1e6, "algorithmic_bytes_each": algo,
             "write_gbs": algo / t_w / 1e9, "read_gbs": algo / t_r / 1e9}
 
 
@@ -316,7 +334,11 @@ def main():
     ap.add_argument("--window", type=int, default=0, help="window-attention: keys a row looks back (0: all)")
     ap.add_argument("--sinks", type=int, default=0, help="window-attention: first keys that stay visible")
     ap.add_argument("--rows-per-stream", type=int, default=1, help="window-attention: consecutive rows of a stream")
+    ap.add_argument("--max-ctx", type=int, default=0, help="window-attention: bound given to the call (0: the longest)")
+    ap.add_argument("--heads", type=int, nargs=3, default=[16, 8, 128], help="window-attention: query heads, KV heads, head_dim")
     ap.add_argument("--tokens", type=int, default=501, help="kv-q4: tokens written and read")
+    ap.add_argument("--dtype", choices=["float16", "bfloat16", "float32"], default="float16", help="kv-q4: type of the rows")
+    ap.add_argument("--scattered", action="store_true", help="kv-q4: one layer, a token in each block (a decode step)")
     ap.add_argument("--chunk", type=int, default=1, help="code2wav: frames per stream per call")
     ap.add_argument("--plain", action="store_true", help="gemm: plain bf16 activations (no lo operand)")
     a = ap.parse_args()
@@ -326,9 +348,9 @@ def main():
         r = bench_prefill_attention(a.streams, a.prefill_chunk, a.past, a.launches, split=a.split)
     elif a.what == "window-attention":
         r = bench_window_attention(a.kv, a.rows, a.rows_per_stream, a.ctx_mean, a.ctx_spread, a.window, a.sinks,
-                                   a.launches)
+                                   a.launches, a.max_ctx, *a.heads)
     elif a.what == "kv-q4":
-        r = bench_kv_q4(a.tokens, a.launches)
+        r = bench_kv_q4(a.tokens, a.launches, a.dtype, a.scattered)
     elif a.what == "code2wav":
         r = bench_code2wav(a.rows, a.launches, chunk=a.chunk)
     else:
