@@ -225,7 +225,13 @@ def stream_ptr(stream=None):
     return stream.cuda_stream
 
 
+# not part of torch's documented interface: None in a release that drops it
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def raw_stream(device: int) -> int:
     """Handle of the current stream of a device (without the ``torch.cuda.Stream`` object around it, which
-    costs 3 us of host time a launch)."""
-    return torch._C._cuda_getCurrentRawStream(device)
+    costs 3 us of host time a launch, where torch offers that)."""
+    if _current_raw_stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _current_raw_stream(device)
