@@ -170,6 +170,39 @@ def test_write_groups_that_saturate_near_the_top():
     _same_bytes(cache.cpu().numpy(), want, 128)
 
 
+def test_first_chunk_of_a_process_inside_a_capture():
+    """The split of a tile's keys asks the card what it holds: also when the first call is captured."""
+    code = """
+import torch
+from test_stateful_b200 import ops
+pools = [torch.zeros(100, 1, 2, 2, 9 * 128, dtype=torch.uint8, device="cuda"),
+         torch.randn(100, 1, 2, 2, 16, 128, device="cuda").half()]
+k = torch.randn(1600, 2, 128, device="cuda"); m = torch.arange(1600, dtype=torch.int32, device="cuda")
+q = torch.randn(200, 4, 128, device="cuda"); t = torch.arange(100, dtype=torch.int32, device="cuda").view(1, 100)
+z = torch.zeros(200, dtype=torch.int32, device="cuda"); c = torch.arange(1401, 1601, dtype=torch.int32, device="cuda")
+def step():
+    ops.kv_write_q4(pools[0], k, -k, m)
+    return (ops.paged_attention_q4(q, pools[0], 0, t, z, c, 1600, rows_per_stream=200),
+            ops.paged_attention_window(q, pools[1], 0, t, z, c, 1600, 0, rows_per_stream=200))
+torch.cuda.synchronize()
+s = torch.cuda.Stream()
+with torch.cuda.stream(s):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        a = step()
+    g.replay()
+    s.synchronize()
+for x, y in zip(a, step()):
+    assert torch.isfinite(x).all() and torch.equal(x, y)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for form in ("1", None):
+        env = {k: v for k, v in os.environ.items() if k != "QTTS_WINDOW_TILES"}
+        r = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(env, QTTS_WINDOW_TILES=form) if form else env,
+                           capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+
+
 @pytest.mark.skipif(FORCED is not None, reason="already a forced run")
 @pytest.mark.parametrize("form", ["0", "1"])
 def test_both_chunk_forms(form):
