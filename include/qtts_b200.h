@@ -260,7 +260,22 @@ int qtts_kv_gather_q4(const void* cache, int num_blocks, int num_layers, int kv_
  * row_slot; 1 = decode rows).  block_table [num_slots][max_blocks_per_seq]; a row_slot outside
  * [0, num_slots) gives zeros, a block id outside the pool hides its keys; both are reported by
  * qtts_device_error.  q and kv_pool must be 16-byte aligned.  No scratch: keys of few rows are split
- * over the CTAs of a cluster and folded through distributed shared memory, in a fixed order. */
+ * over the CTAs of a cluster and folded through distributed shared memory, in a fixed order.
+ *
+ * Precision: q to 2^-21 of its row's largest channel, probabilities to 2^-16 of themselves (4 bits) or 2^-21
+ * (fp16) down to 2^-31 of the row's largest, sums in fp32; out is bf16, out_lo (or NULL) the bf16 residual, and the
+ * two together hold 16 bits.  Chunks (rows_per_stream > 1) go through tiles of 8 or of 128 rows, chosen by sizes
+ * (of the whole call: a chunk alone and in a batch may differ in those last bits); tiles of 128 hold 4-bit values to
+ * 2^-18 of their group's largest (or 2^-23).
+ * What is not finite in q, or in K or V of a visible key, makes the rows that see it NaN: V in its channel, or in all
+ * channels where its block also holds keys hidden from some row of the tile; an infinite K may, by the sign of its
+ * score, only lose its weight (a row whose every visible score is -infinity gets zeros).
+ * max_ctx bounds the contexts (which are on the device) for the choice of form and of the split of the keys: a bound
+ * far above them, as a captured graph gives, costs one short stream up to 3 us (500 keys: 6.4 -> 9.2 over 4 bits).
+ * For plain causal attention over the fp16 pool (window 0) at head_dim 128, qtts_paged_attention and
+ * qtts_paged_attention_prefill (two query heads a KV head) are as fast or faster (64 streams of 520 keys 28.7 us, here
+ * 30-32; 8 x 128 rows after 384 19.0, here 25.1); this entry is for windows, sinks, other head counts and
+ * head_dim 64. */
 int qtts_paged_attention_window(const void* q, int R, int rows_per_stream, int num_heads, int kv_heads, int head_dim,
                                 const void* kv_pool, int layer, int num_layers, int block_size, int num_blocks,
                                 const int32_t* block_table, int num_slots, int max_blocks_per_seq,

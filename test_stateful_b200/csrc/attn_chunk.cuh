@@ -17,12 +17,13 @@
 // the bf16 output rounds off.)  4-bit values are pairs too, to 2^-18 of their group's largest.  Products of two
 // low parts are left out.  Sums, maxima and O are fp32.
 //
-// Bound by, a tile of D = 128: fp16 by 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the softmax does
-// around them, next to some 1600 cycles of products (57 an instruction of N = 64 for S, 88 of N = 128 for P V); 4 bits by the
-// products, three for two (2400 cycles; without the third 19.0 us for 20.7), and K and V made fp16 beside
-// them.  A launch adds some 8 us before its first products and after its last.  16 heads over 8, D = 128, B200: 8 x
-// 128 rows after 384, 4 bits 20.7 us (182 TFLOP/s; 16.7 in single halves); 2 x 500 rows under a window of 256,
-// fp16 21.1 us (102 TFLOP/s; 19.6).  4 bits with the scales on P and on S instead, codes alone in the products: 38.8.
+// Bound by, a tile of D = 128: fp16 by 128 x 64 exponentials (512 cycles at 16 a cycle and SM) and what the
+// softmax does around them, next to some 1600 cycles of products (57 an instruction of N = 64 for S, 88 of
+// N = 128 for P V), and by the copies of K and V; 4 bits by the products, three for two (2400 cycles; without the
+// third 19.0 us for 20.7), and K and V made fp16 beside them.  A launch adds some 8 us before its first
+// products and after its last.  16 heads over 8, D = 128, B200: 8 x 128 rows after 384, 4 bits 20.7 us (182
+// TFLOP/s; 16.7 in single halves), fp16 25.1 (K and V from HBM); 2 x 500 rows under a window of 256, fp16 21.1 us
+// (102 TFLOP/s; 19.6).  4 bits with the scales on P and on S instead, codes alone in the products: 38.8.
 // Every wait is bounded.
 #pragma once
 
@@ -75,7 +76,7 @@ struct ChunkLayout {
     static constexpr int NW = D / 64;
     static constexpr int NP = FMT == kWinQ4 ? 2 : 1;  // fp16 numbers a value of K or V is held in
     static constexpr int ST = FMT == kWinQ4 ? 2 : 4;  // stages of fp16 tiles
-    static constexpr int RAW = FMT == kWinQ4 ? 3 : 0; // tiles of codes on their way (cp.async), before they are turned into fp16
+    static constexpr int RAW = FMT == kWinQ4 ? 3 : 0; // tiles of codes on their way (cp.async), not yet turned into fp16
     static constexpr int PANEL = 64 * 128;            // 64 keys x 64 channels
     static constexpr int PART_KV = NW * PANEL;        // high or low parts of K or V
     static constexpr int STAGE = 2 * NP * PART_KV;    // K's parts, V's parts
@@ -394,7 +395,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const float a = ex2_approx(fmaf(v[32 * c + 2 * k], sf, -mu)), b = ex2_approx(fmaf(v[32 * c + 2 * k + 1], sf, -mu));
+                    const float a = ex2_approx(fmaf(v[32 * c + 2 * k], sf, -mu));
+                    const float b = ex2_approx(fmaf(v[32 * c + 2 * k + 1], sf, -mu));
                     s4[k & 3] += a + b;
                     split_h2(a, b, hi[k], lo[k]);
                 }
@@ -412,11 +414,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_attn_chunk_kernel(cons
     } else if (warp < 12) {
         // ------------------------------------------------------------------ K (is_v 0) or V: block `w4` of each tile
         if constexpr (FMT == kWinQ4) {
-            // Nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as two fp16 pairs, high + low = half of code * scale + zero (half,
-            // so that values past 65504 fit).  With g = 2^-9 of the power of two below the group's largest value M,
-            // scale and zero are multiples of g (sh, zh) and what those leave (sl, zl): the high part is exact, a
-            // multiple of g / 2 below 2^11 of them, and the low part, below 4 g, rounds: the value is off by at most 2^-18 of
-            // M (2^-23 where M is below 2^-5).
+            // Nibbles (0, 4), (1, 5), (2, 6), (3, 7) of a word as two fp16 pairs, high + low = half of code * scale +
+            // zero (half, so that values past 65504 fit).  With g = 2^-9 of the power of two below the group's
+            // largest value M, scale and zero are multiples of g (sh, zh) and what those leave (sl, zl): the high
+            // part is exact, a multiple of g / 2 below 2^11 of them, and the low part, below 4 g, rounds: the value
+            // is off by at most 2^-18 of M (2^-23 where M is below 2^-5).
             auto values = [&](uint32_t x, __half2 sh, __half2 sl, __half2 zh, __half2 zl, uint4& hi, uint4& lo) {
                 uint32_t *oh = &hi.x, *ol = &lo.x;
 #pragma unroll

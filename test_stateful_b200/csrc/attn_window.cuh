@@ -29,10 +29,10 @@
 // of K tokens g and g + 8 the channels 64 w + 16 t .. + 15, of V tokens 2 t, 2 t + 1, 2 t + 8,
 // 2 t + 9 the channels 64 w + 8 g .. + 7.
 //
-// Bound by (16 heads over 8, D = 128, B200): fp16 by HBM, 64 x 4096 keys 172 us (6.25 TB/s); 4 bits by the
-// integer pipe next to HBM, the same keys 64 us (4.7 TB/s).  A decode step of one wave by latencies (block
-// ids, first copies, the longest row): 64 streams of 260 .. 780 keys at 4 bits 17 us, under a window of 72 +
-// 4 over fp16 12 us.
+// Bound by (16 heads over 8, D = 128, B200): fp16 by HBM, 64 x 4096 keys 173 us (6.2 TB/s); 4 bits by instructions
+// (0.53 of the issue slots, 48% of the integer pipe, 32% of the tensor one) next to HBM, the same keys 68 us
+// (4.4 TB/s).  A decode step of one wave by latencies (block ids, first copies, the longest row): 64 streams of 260
+// .. 780 keys at 4 bits 18.7 us, under a window of 72 + 4 12.1 us over fp16, 8.6 over 4 bits.
 #pragma once
 
 #include <type_traits>
@@ -781,14 +781,15 @@ inline int launch_window_rows_w(const WinParams& p, long long tiles, int splits,
 // How a tile's keys are shared.  16 warps fit an SM over the 4-bit pool, 12 over fp16; all variants
 // fill it, with fewer and larger CTAs the fewer tiles there are: warps of one CTA fold cheaper than
 // CTAs of a cluster.  Beyond the tiles that half-SM CTAs cover, a cluster splits a tile while every
-// warp keeps three blocks.  Measured (us, 16 heads over 8, rows x context, B200), warps x splits:
-//   4 bits  1 x 4000:  4 x 16 7.0   8 x 8 7.5    8 x 4 9.3    2 x 16 8.4
-//          16 x 520:   8 x 1 7.0    4 x 1 7.8    8 x 2 8.7    4 x 4 8.8
-//          64 x 520:   4 x 1 14.3   2 x 1 14.7   8 x 1 18.1   4 x 2 20.9
-//         128 x 520:   2 x 1 23.3   4 x 1 25.6   8 x 1 32.7
-//   fp16    1 x 4000:  6 x 8 9.9    3 x 16 9.7   6 x 4 13.5
-//          64 x 520:   3 x 1 27.3   6 x 1 29.1   2 x 1 29.7   3 x 2 33.3
-//         128 x 520:   3 x 1 48.1   2 x 1 57.3   6 x 1 53.5
+// warp keeps three blocks.  Measured (us, 16 heads over 8, rows x context, B200, K and V from HBM), warps x splits:
+//   4 bits  1 x 4000:  8 x 8 8.0    4 x 16 8.1   8 x 16 9.4   8 x 4 9.9    2 x 16 9.3
+//          16 x 520:   8 x 1 7.8    4 x 1 8.7    4 x 2 9.4    8 x 2 10.2   4 x 4 10.1
+//          64 x 520:   4 x 1 16.1   2 x 1 16.3   8 x 1 19.9   4 x 2 23.0
+//         128 x 520:   2 x 1 26.1   4 x 1 28.3   8 x 1 36.4
+//   fp16    1 x 4000:  6 x 8 10.2   3 x 16 10.5  6 x 16 10.6  6 x 4 14.2
+//          16 x 520:   6 x 1 10.3   6 x 2 11.2   3 x 2 12.0   3 x 1 12.1
+//          64 x 520:   3 x 1 26.9   2 x 1 27.7   6 x 1 28.9   3 x 2 33.2
+//         128 x 520:   3 x 1 48.8   2 x 1 58.0   6 x 1 53.8
 template <int FMT, int D, int SL>
 inline int launch_window_rows(WinParams p, cudaStream_t st) {
     using G = WinChunk<FMT, D>;

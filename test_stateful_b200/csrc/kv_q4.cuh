@@ -180,7 +180,9 @@ __device__ __noinline__ float q4_exact_code(float d, float scale, float inv15) {
 // scale and zero worked out by four threads instead of eight: 30 -> 21 us for 501 tokens of 28 layers).
 constexpr int kQ4Threads = 128, kQ4RowsPerCta = kQ4Threads / 4;
 
-// Bound by instruction issue (0.71 of the slots): 501 tokens of 28 layers 18.5 us (4 TB/s; 8 heads, D = 128).
+// Bound by instructions and the wait for the rows they work on (0.71 of the issue slots), not by HBM: 501 tokens
+// of 28 layers 19.3 us in fp16 (3.8 TB/s), 20.7 in bf16, 22.9 in fp32 (5.7 TB/s; 8 heads, D = 128, rows and pools
+// from HBM); a step's 64 tokens of one layer, each in a block of its own, 3.3 us.
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kQ4Threads) kv_write_q4_kernel(const Q4IoParams p) {
     using L = Q4Layout<D>;
@@ -273,7 +275,8 @@ __global__ void __launch_bounds__(kQ4Threads) kv_write_q4_kernel(const Q4IoParam
     }
 }
 
-// Bound by HBM: 501 tokens of 28 layers 11.7 us (6.3 TB/s; 8 heads, D = 128).
+// Bound by HBM: 501 tokens of 28 layers 13.9 us to fp16 (5.3 TB/s), 13.6 to bf16, 35 to fp32 (3.7 TB/s: 64-byte
+// pieces of rows), 1000 tokens 26.3 to fp16 (5.6 TB/s; 8 heads, D = 128, pools from HBM).
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kQ4Threads) kv_read_q4_kernel(const Q4IoParams p) {
     using L = Q4Layout<D>;

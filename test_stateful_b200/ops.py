@@ -283,7 +283,9 @@ def paged_attention_window(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, b
     L, 2, Hkv, 16, D]`` fp16, ``D`` 64 or 128, any whole ``Hq / Hkv``; rows without a visible key get
     zeros.  ``rows_per_stream`` > 1: the rows are streams of that many consecutive query tokens (a
     prompt chunk), which share the blocks they read.  Returns bf16 ``[R, Hq * D]`` (``out_lo``: its bf16
-    residual)."""
+    residual; together they hold 16 bits, in whichever of its forms the call's sizes choose).  For plain causal
+    attention with two query heads a KV head and ``D`` 128, :func:`paged_attention` and
+    :func:`paged_attention_prefill` are as fast or faster."""
     if kv_pool.dtype is not torch.float16 or kv_pool.dim() != 6 or not kv_pool.is_contiguous():
         raise ValueError("paged_attention_window: a contiguous float16 pool [blocks, layers, 2, kv_heads, 16, head_dim]")
     nb, L, two, H, bs, D = kv_pool.shape
@@ -298,7 +300,8 @@ def paged_attention_q4(q: torch.Tensor, cache: torch.Tensor, layer: int, block_t
                        rows_per_stream: int = 1, out: Optional[torch.Tensor] = None,
                        out_lo: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`paged_attention_window` over a 4-bit pool ``cache [blocks, L, 2, Hkv, 9 D]`` (uint8, written by
-    :func:`kv_write_q4`); every key is visible by default."""
+    :func:`kv_write_q4`); every key is visible by default.  Values enter as ``code * scale + zero``, unrounded or
+    (128-row tiles of prompt chunks) to 2^-18 of their group's largest."""
     return _window_attention("paged_attention_q4", _lib.load().qtts_paged_attention_q4, q, cache, _q4_dims(cache), layer,
                              block_table, row_slot, row_ctx, max_ctx, window, sinks, rows_per_stream, out, out_lo)
 
