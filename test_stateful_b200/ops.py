@@ -219,6 +219,8 @@ def kv_read_q4(cache: torch.Tensor, slot_mapping: torch.Tensor, layer: int = 0, 
     for st in (ks, vs):
         if (n > 1 and not st[0]) or (n_layers > 1 and k.dim() == 4 and not st[1]) or (H > 1 and not st[2]):
             raise ValueError("kv_read_q4: k and v must not be broadcast tensors")
+    if n and k.data_ptr() == v.data_ptr():
+        raise ValueError("kv_read_q4: k and v must not be the same memory")
     _launch(dev, "kv_read_q4", _lib.load().qtts_kv_read_q4, cache.data_ptr(), nb, L, H, D, k.data_ptr(), v.data_ptr(), dt,
             ks, vs, layer, n_layers, slot_mapping.data_ptr(), n)
     return k, v
@@ -268,6 +270,8 @@ def _window_attention(what, fn, q, kv, dims, layer, block_table, row_slot, row_c
     if out_lo is not None and (out_lo.dtype is not torch.bfloat16 or out_lo.numel() != R * Hq * D
                                or not out_lo.is_contiguous()):
         raise ValueError(f"{what}: out_lo must be contiguous bfloat16 [{R}, {Hq * D}]")
+    if out_lo is not None and R and out_lo.data_ptr() == out.data_ptr():
+        raise ValueError(f"{what}: out and out_lo must not be the same memory")
     _launch(dev, what, fn, q.data_ptr(), R, rows_per_stream, Hq, H, D, kv.data_ptr(), layer, L, 16, nb,
             block_table.data_ptr(), slots, mbps, row_slot.data_ptr(), row_ctx.data_ptr(), max_ctx, window, sinks,
             out.data_ptr(), None if out_lo is None else out_lo.data_ptr())

@@ -170,6 +170,22 @@ def test_write_groups_that_saturate_near_the_top():
     _same_bytes(cache.cpu().numpy(), want, 128)
 
 
+def test_outputs_that_are_one_memory_are_refused():
+    """Both outputs in one tensor would be a mixture of the two."""
+    cache = _new_cache(2, 1, 2, 64)
+    m = torch.arange(3, dtype=torch.int32, device=DEV)
+    rows = torch.zeros(3, 2, 64, device=DEV)
+    q = torch.zeros(3, 4, 64, device=DEV)
+    t = torch.zeros(3, 2, dtype=torch.int32, device=DEV)
+    out = torch.zeros(3, 256, dtype=torch.bfloat16, device=DEV)
+    pool = torch.zeros(2, 1, 2, 2, 16, 64, dtype=torch.float16, device=DEV)
+    for call in (lambda: ops.kv_read_q4(cache, m, k=rows, v=rows),
+                 lambda: ops.paged_attention_q4(q, cache, 0, t, m, m, 32, out=out, out_lo=out),
+                 lambda: ops.paged_attention_window(q, pool, 0, t, m, m, 32, 8, out=out, out_lo=out.view(-1))):
+        with pytest.raises(ValueError, match="same memory"):
+            call()
+
+
 def test_first_chunk_of_a_process_inside_a_capture():
     """The split of a tile's keys asks the card what it holds: also when the first call is captured."""
     code = """
